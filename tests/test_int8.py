@@ -1,0 +1,673 @@
+"""8-bit serving (ops/int8.py) against definitions in 64 bits.
+
+Tolerances.  An integer of a row is the nearest to 127 y / max|y|, where the kernel's y and maximum are off by a relative
+error e each: |q - 127 y / max| <= 1/2 + 127 * 2 e.  For plain rows e is one rounding of 127 / max (2^-24); for a norm
+h w is rounded too (2^-23 is enough for both); behind a gate the exponential's argument z log2(e) is off by |z| 2^-24, with
+the exponential's and the reciprocal's last places below 2^-18 for |z| < 50; a rotated pair is off by 3 roundings of its
+larger input, which is at most sqrt 2 of the largest rotated one (2^-21).  Scales are fp32 with the same errors; a norm's has
+the sum of squares' (H / 64 + 16 additions at most in a row, half of it by the root: 2^-17 at the sizes here).
+A product's integer sum is exact, then rounded to fp32 (2^-24), multiplied twice and added once: 2^-22 of its terms; bf16
+adds half a step, 2^-8.  Attention rounds each weight to bf16 (2^-8 of sum p |v|), its result (2^-8), and its scores
+accumulate 128 terms in fp32 (130 2^-24 of sum |q k|, twice in a weight's relative error)."""
+import math
+
+import pytest
+import torch
+
+from k8s_llm_rca_amd.ops import attention as A
+from k8s_llm_rca_amd.ops import int8 as Q
+
+BF, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+D = 128
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def randn(g, *shape, dtype=F32, device="cpu"):
+    return torch.randn(*shape, generator=g).to(dtype).to(device)
+
+
+def check_rows(q, scale, y, e, es=2.0 ** -22):
+    """q and scale against rows y in fp64."""
+    y, q, scale = y.double().cpu(), q.double().cpu(), scale.double().cpu()
+    top = y.abs().amax(-1)
+    fine = torch.isfinite(top)
+    zero = fine & (top < Q.TINY)
+    live = fine & ~zero
+    assert bool(torch.isnan(scale[~fine]).all()) and not q[~fine].any()
+    assert not scale[zero].any() and not q[zero].any()
+    real = 127 * y[live] / top[live][:, None]
+    assert float((q[live] - real).abs().max() if live.any() else 0) <= 0.5 + 254 * e
+    assert bool(((scale[live] - top[live] / 127).abs() <= (es + 2 * e) * top[live] / 127).all())
+
+
+# ------------------------------------------------------------------ rows
+WIDTHS = [16, 48, 128, 2032, 2048, 2064, 4096, 8192, 8208, 14336, 32768, 33008]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T,H", [(1 + i % 5, h) for i, h in enumerate(WIDTHS)] + [(301, 80), (67, 4096)])
+def test_rows(device, dtype, T, H):
+    x = randn(gen(H + T), T, H, dtype=dtype)
+    x[0] *= 1000
+    if T > 2:
+        x[1] = 0
+        x[2] *= 2.0 ** -110
+    q, s = Q.quantize_rows(x.to(device))
+    check_rows(q, s, x, 2.0 ** -24)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T,H", [(1 + i % 5, h) for i, h in enumerate(WIDTHS)] + [(301, 80), (67, 4096)])
+def test_gate(device, dtype, T, H):
+    gu = randn(gen(H), T, 2 * H, dtype=dtype)
+    gu[:, :H] *= 4
+    q, s = Q.silu_mul_int8(gu.to(device))
+    g, u = gu.double().chunk(2, -1)
+    check_rows(q, s, g * torch.sigmoid(g) * u, 2.0 ** -18)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("T,H", [(1 + i % 5, h) for i, h in enumerate(WIDTHS)] + [(301, 80), (67, 4096)])
+def test_norm(device, dtype, residual, T, H):
+    g = gen(H)
+    x, w = randn(g, T, H, dtype=dtype), (1 + 0.1 * randn(g, H)).to(dtype)
+    r = randn(g, T, H, dtype=dtype) if residual else None
+    rd = r.clone().to(device) if residual else None
+    q, s = Q.rmsnorm_int8(x.to(device), w.to(device), 1e-5, residual=rd)
+    h = x.double()
+    if residual:
+        want = (x.float() + r.float()).to(dtype)
+        assert torch.equal(rd.cpu(), want)
+        h = want.double()
+    y = h * w.double() / (h.square().mean(-1, keepdim=True) + 1e-5).sqrt()
+    check_rows(q, s, y, 2.0 ** -22, 2.0 ** -17)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("H", [128, 4096, 16384, 33008])
+def test_rows_that_hold_no_number(device, H):
+    x = randn(gen(1), 5, H, dtype=BF)
+    x[0, H // 2] = math.nan
+    x[1, 3] = math.inf
+    x[2, H - 1] = -math.inf
+    x[3] = 0
+    for q, s in (Q.quantize_rows(x.to(device)), Q.rmsnorm_int8(x.to(device), torch.ones(H, dtype=BF, device=device), 1e-5)):
+        assert torch.isnan(s[:3]).all() and not q[:4].any() and s[3] == 0 and torch.isfinite(s[4]) and q[4].any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rows_strides_and_outs(device):
+    g = gen(3)
+    whole = randn(g, 9, 400, dtype=BF, device=device)
+    x = whole[::2, 7:7 + 128]                                 # rows that start anywhere
+    out = torch.full((5, 160), 77, dtype=torch.int8, device=device)
+    s = torch.empty(5, device=device)
+    q, s2 = Q.quantize_rows(x, out=out[:, :128], scale=s)
+    assert s2.data_ptr() == s.data_ptr() and q.data_ptr() == out.data_ptr()
+    check_rows(q, s, x.cpu(), 2.0 ** -24)
+    assert bool((out[:, 128:] == 77).all())
+    e, es = Q.quantize_rows(x[:0])
+    assert e.shape == (0, 128) and es.shape == (0,)
+    col = whole.t()[:16, :9].t()                              # columns one behind another
+    q, s = Q.quantize_rows(col)
+    check_rows(q, s, col.cpu(), 2.0 ** -24)
+
+
+# ------------------------------------------------------------------ products
+def product_case(device, M, N, K, dtype=BF, bias=False, seed=0):
+    g = gen(seed + M + N + K)
+    x = torch.randint(-127, 128, (M, K), generator=g, dtype=torch.int8).to(device)
+    w = torch.randint(-127, 128, (N, K), generator=g, dtype=torch.int8).to(device)
+    xs, ws = (0.001 + torch.rand(n, generator=g) for n in (M, N))
+    b = 100 * K * randn(g, N) if bias else None
+    return x, xs.to(device), w, ws.to(device), None if b is None else b.to(device)
+
+
+def check_product(y, x, xs, w, ws, b):
+    x, xs, w, ws = (t.double() for t in (x, xs, w, ws))
+    want = x @ w.T * xs[:, None] * ws
+    size = want.abs()
+    if b is not None:
+        want, size = want + b.double(), size + b.double().abs()
+    tol = 2.0 ** -22 * size + (2.0 ** -8 * want.abs() if y.dtype == BF else 0)
+    assert bool(((y.double() - want).abs() <= tol).all())
+
+
+SIZES = [(1, 1, 16), (1, 6144, 4096), (2, 17, 48), (5, 33, 80), (16, 64, 64), (17, 100, 1040), (31, 515, 144), (33, 256, 512),
+         (48, 1000, 4096), (64, 47, 4112), (65, 129, 256), (100, 300, 2064), (128, 128, 128), (129, 257, 400), (200, 1030, 1024),
+         (256, 256, 256), (257, 513, 272), (300, 4096, 512), (513, 1000, 16), (1000, 777, 1152), (1111, 2048, 640), (2050, 300, 2048)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", SIZES)
+@pytest.mark.parametrize("dtype,bias", [(BF, False), (F32, True)])
+def test_product(M, N, K, dtype, bias):
+    args = product_case("cuda", M, N, K, dtype, bias)
+    check_product(Q.linear_int8(*args[:4], bias=args[4], out_dtype=dtype), *args)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 1, 16), (3, 5, 48), (33, 17, 4096)])
+def test_product_plain(M, N, K):
+    for dtype, bias in ((BF, False), (F32, True)):
+        args = product_case("cpu", M, N, K, dtype, bias)
+        check_product(Q.linear_int8(*args[:4], bias=args[4], out_dtype=dtype), *args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K", [(1, Q.MAX_K), (40, 65536), (130, Q.MAX_K), (300, Q.MAX_K)])
+def test_product_of_the_longest_rows_does_not_overflow(M, K):
+    x = torch.full((M, K), -128, dtype=torch.int8, device="cuda")
+    w = torch.full((20, K), -128, dtype=torch.int8, device="cuda")
+    w[1::2] = 127
+    one = torch.ones(max(M, 20), device="cuda")
+    y = Q.linear_int8(x, one[:M], w, one[:20], out_dtype=F32)
+    assert bool((y[:, 0::2] == float(128 * 128 * K)).all() and ((y[:, 1::2] + 128 * 127 * K).abs() <= 2.0 ** -24 * 128 * 127 * K).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 20, 70, 300, 600])
+def test_a_row_does_not_depend_on_the_rows_beside_it(M):
+    x, xs, w, ws, b = product_case("cuda", 1200, 1100, 1040, bias=True)
+    whole = Q.linear_int8(x, xs, w, ws, bias=b)
+    assert torch.equal(Q.linear_int8(x[37:37 + M], xs[37:37 + M], w, ws, bias=b), whole[37:37 + M])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 40, 150, 700])
+def test_product_strides_and_scales_without_a_number(M):
+    g = gen(M)
+    x = torch.randint(-127, 128, (M, 700), generator=g, dtype=torch.int8).cuda()[:, 5:5 + 320]
+    w = torch.randint(-127, 128, (90, 400), generator=g, dtype=torch.int8).cuda()[:, 16:16 + 320]
+    xs, ws = torch.rand(M, generator=g).cuda(), torch.rand(90, generator=g).cuda()
+    xs[M // 2] = math.nan
+    big = torch.full((M + 1, 101), 7.0, dtype=BF, device="cuda")
+    y = Q.linear_int8(x, xs, w, ws, out=big[:M, 3:93])
+    assert bool(torch.isnan(y[M // 2]).all())
+    keep = [m for m in range(M) if m != M // 2]
+    check_product(y[keep], x[keep], xs[keep], w, ws, None)
+    assert bool((big[:, :3] == 7).all() and (big[:, 93:] == 7).all() and (big[M] == 7).all())
+
+
+@pytest.mark.gpu
+def test_product_of_rows_far_apart():
+    far = torch.empty(20 << 27, dtype=torch.int8, device="cuda")
+    x = far.as_strided((20, 64), (1 << 27, 1))
+    w = far.as_strided((20, 64), (1 << 27, 1), 4096)
+    g = gen(5)
+    x.copy_(torch.randint(-127, 128, (20, 64), generator=g, dtype=torch.int8))
+    w.copy_(torch.randint(-127, 128, (20, 64), generator=g, dtype=torch.int8))
+    one = torch.ones(20, device="cuda")
+    check_product(Q.linear_int8(x, one, w, one, out_dtype=F32), x, one, w, one, None)
+    many = x.repeat(7, 1)
+    ones = torch.ones(140, device="cuda")
+    check_product(Q.linear_int8(many, ones, w, one, out_dtype=F32), many, ones, w, one, None)
+
+
+# ------------------------------------------------------------------ the cache
+def table(n):
+    return A.rope_cos_sin(n, device="cpu")
+
+
+def write_case(T, nq, nkv, BS, slots, seed=0, pad=0):
+    g = gen(seed + T + nq)
+    qkv = randn(g, T, (nq + 2 * nkv) * D + pad, dtype=BF)
+    pos = torch.randint(0, 500, (T,), generator=g, dtype=torch.int32)
+    return qkv, pos, torch.as_tensor(slots, dtype=torch.int32)
+
+
+def noise(cache, seed=9):
+    g = gen(seed)
+    dev = cache.k.device
+    for t in (cache.k, cache.v):
+        t.copy_(torch.randint(-127, 128, t.shape, generator=g, dtype=torch.int8).to(dev))
+    for t in (cache.k_scale, cache.v_scale):
+        t.copy_(torch.rand(t.shape, generator=g).to(dev))
+    return cache
+
+
+def runs(*parts):
+    return [s for a, b in parts for s in range(a, b)]
+
+
+WRITES = [
+    (4, 1, 64, [130]), (8, 2, 64, [5, -1, 64 * 3 + 63, 64 * 7, 0, -1]), (32, 8, 64, runs((70, 70 + 129), (3, 9)) + [-1, -1]),
+    (4, 4, 128, runs((128 * 4 + 1, 128 * 5 + 17), (0, 64))), (6, 2, 64, list(range(64 * 8 - 1, -1, -3))), (1, 1, 64, runs((0, 64 * 8))),
+    (8, 1, 192, runs((190, 195), (16, 32), (192 * 7, 192 * 8))), (2, 2, 64, [64 * 8, 10 ** 6, 1]), (10, 2, 64, runs((61, 200)))]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("nq,nkv,BS,slots", WRITES)
+def test_write(device, nq, nkv, BS, slots):
+    T = len(slots)
+    qkv, pos, at = write_case(T, nq, nkv, BS, slots, pad=16)
+    cs = table(512)
+    cache = noise(Q.Int8KV.empty(8, nkv, BS, device))
+    before = [t.clone().cpu() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    mine = qkv.clone().to(device)
+    Q.rope_kv_write_int8(mine, pos.to(device), cs.to(device), at.to(device), cache, nq, nkv)
+    x = qkv[:, :(nq + 2 * nkv) * D].double().view(T, -1, D)
+    c, s = cs.double()[pos.long()][:, None].chunk(2, -1)
+    a, b = x.chunk(2, -1)
+    turned = torch.cat([a * c - b * s, b * c + a * s], -1)
+    got = mine.cpu().double()
+    size = x[:, :nq].abs().amax(-1, keepdim=True)
+    assert bool(((got[:, :nq * D].view(T, nq, D) - turned[:, :nq]).abs() <= 2.0 ** -8 * turned[:, :nq].abs() + 2.0 ** -22 * size).all())
+    assert torch.equal(got[:, nq * D:], qkv[:, nq * D:].double())
+    k, v, ks, vs = (t.cpu() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale))
+    kept = [(t, p) for t, p in enumerate(slots) if 0 <= p < 8 * BS]
+    for t, p in kept:
+        check_rows(k[p // BS, :, p % BS], ks[p // BS, :, p % BS], turned[t, nq:nq + nkv], 2.0 ** -21)
+        check_rows(v[p // BS, :, :, p % BS], vs[p // BS, :, p % BS], x[t, nq + nkv:], 2.0 ** -24)
+    touched = torch.zeros(8, BS, dtype=torch.bool)
+    for _, p in kept:
+        touched[p // BS, p % BS] = True
+    for t, old in zip((k, v.transpose(2, 3), ks, vs), (before[0], before[1].transpose(2, 3), before[2], before[3])):
+        rest = ~touched
+        assert torch.equal(t.transpose(1, 2)[rest], old.transpose(1, 2)[rest])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_write_without_slots_and_without_rows(device):
+    qkv, pos, _ = write_case(3, 4, 2, 64, [0, 1, 2])
+    cs = table(512).to(device)
+    cache = noise(Q.Int8KV.empty(2, 2, 64, device))
+    old = [t.clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    one, two = qkv.clone().to(device), qkv.clone().to(device)
+    Q.rope_kv_write_int8(one, pos.to(device), cs, None, cache, 4, 2)
+    assert all(torch.equal(a, b) for a, b in zip(old, (cache.k, cache.v, cache.k_scale, cache.v_scale)))
+    Q.rope_kv_write_int8(two, pos.to(device), cs, torch.arange(3, dtype=torch.int32, device=device), cache, 4, 2)
+    assert torch.equal(one, two) and not torch.equal(one.cpu()[:, :512], qkv[:, :512])
+    Q.rope_kv_write_int8(one[:0], pos.to(device)[:0], cs, None, cache, 4, 2)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_write_of_heads_that_hold_no_number(device):
+    qkv, pos, at = write_case(70, 2, 2, 64, range(64, 134))
+    qkv[3, 2 * D + 5] = math.inf
+    qkv[4, 5 * D + 7] = math.nan
+    qkv[5, 4 * D:5 * D] = 0
+    cache = noise(Q.Int8KV.empty(4, 2, 64, device))
+    Q.rope_kv_write_int8(qkv.clone().to(device), pos.to(device), table(512).to(device), at.to(device), cache, 2, 2)
+    k, v, ks, vs = (t.cpu() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale))
+    assert torch.isnan(ks[1, 0, 3]) and not k[1, 0, 3].any() and torch.isfinite(ks[1, 1, 3])
+    assert torch.isnan(vs[1, 1, 4]) and not v[1, 1, :, 4].any() and torch.isfinite(vs[1, 0, 4])
+    assert vs[1, 0, 5] == 0 and not v[1, 0, :, 5].any()
+    assert torch.isfinite(ks[1:3].flatten()).sum() == 2 * 2 * 64 - 1
+
+
+# ------------------------------------------------------------------ attention
+def attn_case(device, lens, nq, nkv, BS=64, seed=0, spread=1.0, extra=0, NB=None):
+    """lens: (new rows, context) of each sequence; pages behind a context's end and pages of no one hold NaN scales."""
+    g = gen(seed + sum(a * 7 + b for a, b in lens) + nq)
+    counts = [-(-max(c, 0) // BS) for _, c in lens]
+    NB = NB or sum(counts) + 2
+    cache = noise(Q.Int8KV.empty(NB, nkv, BS, device), seed)
+    cache.k_scale.mul_(0.02).add_(0.005)
+    cache.v_scale.mul_(0.02).add_(0.005)
+    order = torch.randperm(NB, generator=g)
+    bt = torch.zeros(len(lens), max(max(counts), 1) + extra, dtype=torch.int32)
+    live = torch.zeros(NB, BS, dtype=torch.bool)
+    at = 0
+    for i, (n, (_, c)) in enumerate(zip(counts, lens)):
+        bt[i, :n] = order[at:at + n].int()
+        for j in range(n):
+            live[order[at + j], :c - j * BS] = True
+        at += n
+    for t in (cache.k_scale, cache.v_scale):
+        t.transpose(1, 2)[~live.to(device)] = math.nan
+    T = sum(a for a, _ in lens)
+    q = (spread * randn(g, T, nq * D + 32)).to(BF).to(device)
+    starts = [0]
+    for a, _ in lens:
+        starts.append(starts[-1] + a)
+    decode = all(a == 1 for a, _ in lens)
+    ctx = [c for _, c in lens]
+    meta = A.AttnMeta(block_tables=bt.to(device), ctx_lens=torch.tensor(ctx, dtype=torch.int32, device=device),
+                      q_start=torch.tensor(starts, dtype=torch.int32, device=device), num_seqs=len(lens), decode=decode)
+    return q, cache, meta, starts, ctx
+
+
+def planned(meta, starts, ctx, nq, nkv, BS, part=None, device="cuda"):
+    if meta.decode:
+        return A.attach_decode_plan(meta, ctx, nq, nkv, BS, device, part=part)
+    return A.attach_plan(meta, A.plan_prefill(starts, nq // nkv, BS, ctx, nkv), device)
+
+
+def check_attention(out, q, cache, meta, starts, ctx, nq, nkv, scale):
+    G, BS = nq // nkv, cache.k.shape[2]
+    for s, c in enumerate(ctx):
+        n = starts[s + 1] - starts[s]
+        if n == 0:
+            continue
+        y = out[starts[s]:starts[s + 1]].double().view(n, nq, D)
+        at = meta.block_tables[s, :-(-max(c, 0) // BS)].long()
+        for h in range(nq):
+            j = h // G
+            if c <= 0:
+                assert not y[:, h].any()
+                continue
+            k = (cache.k[at, j].double() * cache.k_scale[at, j].double()[..., None]).reshape(-1, D)[:c]
+            v = (cache.v[at, j].double() * cache.v_scale[at, j].double()[:, None]).transpose(1, 2).reshape(-1, D)[:c]
+            x = q[starts[s]:starts[s + 1], h * D:(h + 1) * D].double()
+            sc = x @ k.T * scale
+            hidden = torch.arange(c, device=sc.device) > (c - n + torch.arange(n, device=sc.device))[:, None]
+            p = torch.softmax(sc.masked_fill(hidden, -math.inf), -1).masked_fill(hidden, 0.0)
+            want = p @ v
+            off = 2 * 130 * 2.0 ** -24 * (x.abs() @ k.abs().T * scale).amax() + 2.0 ** -20
+            tol = (2.0 ** -8 + off) * (p @ v.abs()) + 2.0 ** -8 * want.abs() + 1e-30
+            assert bool(((y[:, h] - want).abs() <= tol).all()), (s, h, float(((y[:, h] - want).abs() / tol).max()))
+
+
+REPLIES = [
+    ([(1, 1)], 4, 1, 64), ([(1, 63), (1, 64), (1, 65), (1, 2)], 8, 2, 64), ([(1, 700), (1, 0), (1, 129), (1, 1)], 32, 8, 64),
+    ([(1, 1000), (1, 127)], 8, 8, 128), ([(1, 5003)], 32, 8, 64), ([(1, 900)] * 3, 12, 4, 192), ([(1, 300)], 16, 1, 64),
+    ([(1, 2000 - 13 * i) for i in range(40)], 10, 2, 64), ([(1, 0)], 4, 2, 64)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lens,nq,nkv,BS", REPLIES)
+@pytest.mark.parametrize("part", [None, 64, 320])
+def test_reply(device, lens, nq, nkv, BS, part):
+    q, cache, meta, starts, ctx = attn_case(device, lens, nq, nkv, BS)
+    if device == "cuda":
+        planned(meta, starts, ctx, nq, nkv, BS, part)
+    out = torch.full((len(lens), nq * D + 8), 7.0, dtype=BF, device=device)
+    Q.paged_attention_int8(q, cache, meta, nq, nkv, 0.09, out=out[:, :nq * D])
+    check_attention(out[:, :nq * D].contiguous(), q, cache, meta, starts, ctx, nq, nkv, 0.09)
+    assert bool((out[:, nq * D:] == 7).all())
+
+
+CHUNKS = [
+    ([(2, 2)], 4, 1, 64), ([(5, 5), (1, 70), (64, 64), (3, 200)], 8, 2, 64), ([(130, 700), (1, 1), (65, 65)], 32, 8, 64),
+    ([(100, 100)], 8, 8, 128), ([(300, 1500)], 16, 1, 64), ([(0, 90), (17, 130), (0, 0), (2, 64)], 12, 4, 192),
+    ([(33, 4001)], 32, 8, 64), ([(700, 700), (50, 1000)], 10, 2, 64), ([(40, 333)], 4, 4, 64), ([(9, 600)], 17, 1, 64),
+    ([(20, 40)], 100, 1, 64)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lens,nq,nkv,BS", CHUNKS)
+def test_chunk(device, lens, nq, nkv, BS):
+    q, cache, meta, starts, ctx = attn_case(device, lens, nq, nkv, BS)
+    if device == "cuda":
+        planned(meta, starts, ctx, nq, nkv, BS)
+    out = Q.paged_attention_int8(q, cache, meta, nq, nkv, 0.09)
+    check_attention(out, q, cache, meta, starts, ctx, nq, nkv, 0.09)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rows_in_front_of_their_context_are_zero(device):
+    """More new rows than the context has: the first ones see no key."""
+    q, cache, meta, starts, ctx = attn_case(device, [(10, 6), (70, 3)], 8, 2)
+    if device == "cuda":                                       # (a plan of whole key ranges: the splitting one wants a key a tile)
+        A.attach_plan(meta, A.plan_prefill(starts, 4, 64), device)
+    out = Q.paged_attention_int8(q, cache, meta, 8, 2, 0.09)
+    assert not out[:4].any() and not out[10:77].any() and torch.isfinite(out).all() and out[4:10].any(1).all()
+    check_attention(out, q, cache, meta, starts, ctx, 8, 2, 0.09)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[(1, 4000), (1, 517)], [(40, 4000), (90, 517)]])
+@pytest.mark.parametrize("spread", [30.0, 0.0])
+def test_attention_of_sharp_and_flat_scores(lens, spread):
+    q, cache, meta, starts, ctx = attn_case("cuda", lens, 8, 2, spread=spread)
+    planned(meta, starts, ctx, 8, 2, 64)
+    check_attention(Q.paged_attention_int8(q, cache, meta, 8, 2, 0.09), q, cache, meta, starts, ctx, 8, 2, 0.09)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[(1, 300), (1, 300)], [(40, 300), (40, 300)]])
+def test_a_key_without_a_number_reaches_the_rows_that_see_it(lens):
+    q, cache, meta, starts, ctx = attn_case("cuda", lens, 4, 2)
+    planned(meta, starts, ctx, 4, 2, 64)
+    clean = Q.paged_attention_int8(q, cache, meta, 4, 2, 0.09).clone()
+    cache.k_scale[meta.block_tables[0, 4].long(), 1, 290 - 256] = math.nan
+    out = Q.paged_attention_int8(q, cache, meta, 4, 2, 0.09)
+    n = lens[0][0]
+    sees = torch.arange(n, device="cuda") + 300 - n >= 290
+    assert bool(torch.isnan(out[:n][sees][:, 2 * D:]).all())
+    assert torch.equal(out[:n][~sees], clean[:n][~sees]) and torch.equal(out[:, :2 * D], clean[:, :2 * D]) and torch.equal(out[n:], clean[n:])
+
+
+@pytest.mark.gpu
+def test_pages_behind_two_gigabytes():
+    NB = 34000                                               # 8 heads x 64 x 128: 2.2 GB of keys
+    for lens in ([(1, 700)], [(70, 700)]):
+        q, cache, meta, starts, ctx = attn_case("cpu", lens, 8, 8)
+        far = Q.Int8KV.empty(NB, 8, 64, "cuda")
+        n = cache.k.shape[0]
+        for a, b in zip((far.k, far.v, far.k_scale, far.v_scale), (cache.k, cache.v, cache.k_scale, cache.v_scale)):
+            a[NB - n:] = b.cuda()
+        meta.block_tables, meta.ctx_lens, meta.q_start = meta.block_tables.cuda() + (NB - n), meta.ctx_lens.cuda(), meta.q_start.cuda()
+        q = q.cuda()
+        qkv = torch.cat([q[:, :8 * D], torch.randn(len(q), 16 * D, device="cuda").to(BF)], 1).contiguous()
+        own = torch.arange(ctx[0] - len(q), ctx[0], device="cuda")
+        slots = meta.block_tables[0][own // 64] * 64 + own.int() % 64
+        Q.rope_kv_write_int8(qkv, own.int(), table(1024).cuda(), slots.int(), far, 8, 8)
+        planned(meta, starts, ctx, 8, 8, 64)
+        out = Q.paged_attention_int8(qkv, far, meta, 8, 8, 0.09)
+        check_attention(out, qkv, far, meta, starts, ctx, 8, 8, 0.09)
+        del far
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals():
+    x, w = torch.randn(4, 64), torch.ones(64)
+    bad = ValueError
+    with pytest.raises(TypeError):
+        Q.quantize_rows(x.half())
+    with pytest.raises(bad):
+        Q.quantize_rows(x[:, :40])
+    with pytest.raises(bad):
+        Q.quantize_rows(x[0])
+    with pytest.raises(bad):
+        Q.quantize_rows(x, out=torch.empty(4, 64))
+    with pytest.raises(bad):
+        Q.quantize_rows(x, scale=torch.empty(5))
+    with pytest.raises(bad):
+        Q.silu_mul_int8(torch.randn(4, 63))
+    with pytest.raises(bad):
+        Q.silu_mul_int8(torch.randn(4, 48))
+    with pytest.raises(bad):
+        Q.rmsnorm_int8(x, w[:48], 1e-5)
+    with pytest.raises(bad):
+        Q.rmsnorm_int8(x, w.to(BF), 1e-5)
+    with pytest.raises(bad):
+        Q.rmsnorm_int8(x, w, 1e-5, residual=torch.randn(4, 128)[:, ::2])
+    with pytest.raises(bad):
+        Q.rmsnorm_int8(x, w, 1e-5, residual=torch.randn(4, 64).to(BF))
+    leaf = torch.randn(4, 64, requires_grad=True)
+    with pytest.raises(RuntimeError):
+        Q.quantize_rows(leaf)
+    with torch.no_grad():
+        Q.quantize_rows(leaf)
+    q, s = Q.quantize_rows(x)
+    p, t = Q.quantize_rows(torch.randn(8, 64))
+    with pytest.raises(TypeError):
+        Q.linear_int8(x, s, p, t)
+    with pytest.raises(bad):
+        Q.linear_int8(q, t, p, t)
+    with pytest.raises(bad):
+        Q.linear_int8(q, s, p, s)
+    with pytest.raises(bad):
+        Q.linear_int8(q[:, :48], s, p, t)
+    with pytest.raises(bad):
+        Q.linear_int8(q[:, :40], s, p[:, :40], t)
+    with pytest.raises(bad):
+        Q.linear_int8(q, s, p, t, bias=torch.ones(4))
+    with pytest.raises(TypeError):
+        Q.linear_int8(q, s, p, t, out_dtype=torch.float16)
+    with pytest.raises(bad):
+        Q.linear_int8(q, s, p, t, out=torch.empty(4, 9))
+    with pytest.raises(bad):
+        Q.linear_int8(torch.zeros(1, Q.MAX_K + 16, dtype=torch.int8), s[:1], torch.zeros(8, Q.MAX_K + 16, dtype=torch.int8), t)
+
+
+def test_refusals_of_the_cache():
+    bad = ValueError
+    cache = Q.Int8KV.empty(4, 2, 64, "cpu")
+    with pytest.raises(bad):
+        Q.Int8KV.empty(4, 2, 32, "cpu")
+    with pytest.raises(bad):
+        Q.Int8KV(cache.k, cache.k, cache.k_scale, cache.v_scale)
+    with pytest.raises(bad):
+        Q.Int8KV(cache.k, cache.v, cache.k_scale[:2], cache.v_scale)
+    with pytest.raises(bad):
+        Q.Int8KV(cache.k.to(torch.uint8), cache.v, cache.k_scale, cache.v_scale)
+    qkv, pos, at = write_case(3, 4, 2, 64, [1, 2, 3])
+    cs = table(512)
+    for args in ((qkv[:, :-1], pos, cs, at, cache, 4, 2), (qkv, pos.long(), cs, at, cache, 4, 2), (qkv, pos[:2], cs, at, cache, 4, 2),
+                 (qkv, pos, cs, at.long(), cache, 4, 2), (qkv, pos, cs.double(), at, cache, 4, 2), (qkv, pos, cs, at, cache, 4, 1),
+                 (qkv, pos, cs, at, cache, 5, 2), (qkv, pos, cs[:, :64], at, cache, 4, 2)):
+        with pytest.raises(bad):
+            Q.rope_kv_write_int8(*args)
+    q, cache, meta, starts, ctx = attn_case("cpu", [(1, 70), (1, 3)], 4, 2)
+    for args in ((q[:, :256], cache, meta, 4, 2, 1.0), (q, cache, meta, 3, 2, 1.0), (q, cache, meta, 4, 4, 1.0)):
+        with pytest.raises(bad):
+            Q.paged_attention_int8(*args)
+    with pytest.raises(bad):
+        Q.paged_attention_int8(q, cache, meta, 4, 2, 1.0, out=torch.empty(2, 512))
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_device():
+    q, cache, meta, starts, ctx = attn_case("cuda", [(1, 70), (1, 3)], 4, 2)
+    with pytest.raises(ValueError):                            # no plan
+        Q.paged_attention_int8(q, cache, meta, 4, 2, 1.0)
+    with pytest.raises(TypeError):
+        Q.paged_attention_int8(q.float(), cache, meta, 4, 2, 1.0)
+    with pytest.raises(ValueError):
+        Q.paged_attention_int8(q[:, 1:], cache, meta, 4, 2, 1.0)
+    x, s = Q.quantize_rows(torch.randn(4, 64, device="cuda"))
+    with pytest.raises(ValueError):                            # two devices
+        Q.linear_int8(x, s, x.cpu(), s)
+    with pytest.raises(ValueError):                            # a weight's rows that no 16-byte load reaches
+        Q.linear_int8(x[:, :48], s, torch.zeros(4, 65, dtype=torch.int8, device="cuda")[:, 1:49], s)
+
+
+# ------------------------------------------------------------------ together
+class Layer:
+    """A decoder layer in 8 bits, as the module's docstring has it."""
+
+    def __init__(self, H, nq, nkv, inter, NB, device="cuda"):
+        g = gen(77)
+        self.nq, self.nkv, self.scale = nq, nkv, D ** -0.5
+        make = lambda n, k: Q.quantize_rows((randn(g, n, k) * k ** -0.5).to(BF).to(device))  # noqa: E731
+        self.wqkv, self.wo, self.wgu, self.wdown = make((nq + 2 * nkv) * D, H), make(H, nq * D), make(2 * inter, H), make(H, inter)
+        self.n1, self.n2 = ((1 + 0.1 * randn(g, H)).to(BF).to(device) for _ in range(2))
+        self.cs = table(4096).to(device)
+        self.cache = Q.Int8KV.empty(NB, nkv, 64, device)
+
+    def step(self, x, residual, pos, slots, meta):
+        kept = {}
+        kept["y"] = Q.rmsnorm_int8(x, self.n1, 1e-5, residual=residual)
+        kept["qkv0"] = Q.linear_int8(*kept["y"], *self.wqkv)
+        qkv = kept["qkv"] = kept["qkv0"].clone()
+        Q.rope_kv_write_int8(qkv, pos, self.cs, slots, self.cache, self.nq, self.nkv)
+        kept["a"] = Q.paged_attention_int8(qkv, self.cache, meta, self.nq, self.nkv, self.scale)
+        kept["qa"] = Q.quantize_rows(kept["a"])
+        kept["o"] = Q.linear_int8(*kept["qa"], *self.wo)
+        kept["z"] = Q.rmsnorm_int8(kept["o"], self.n2, 1e-5, residual=residual)
+        kept["gu"] = Q.linear_int8(*kept["z"], *self.wgu)
+        kept["act"] = Q.silu_mul_int8(kept["gu"])
+        kept["out"] = Q.linear_int8(*kept["act"], *self.wdown)
+        return kept
+
+
+def layer_meta(chunks, ctx, bt, nq, nkv, device="cuda"):
+    starts = [0]
+    for n in chunks:
+        starts.append(starts[-1] + n)
+    meta = A.AttnMeta(block_tables=bt, ctx_lens=torch.tensor(ctx, dtype=torch.int32, device=device),
+                      q_start=torch.tensor(starts, dtype=torch.int32, device=device), num_seqs=len(chunks), decode=all(n == 1 for n in chunks))
+    pos = torch.cat([torch.arange(c - n, c) for n, c in zip(chunks, ctx)])
+    seq = torch.repeat_interleave(torch.arange(len(chunks)), torch.tensor(chunks))
+    slots = bt.cpu()[seq, pos // 64].long() * 64 + pos % 64
+    return planned(meta, starts, ctx, nq, nkv, 64), starts, pos.int().to(device), slots.int().to(device)
+
+
+@pytest.mark.gpu
+def test_a_layer_over_prompts_and_replies():
+    """Two prompt chunks and three replies of three threads; every operator against its definition on what it was given."""
+    H, nq, nkv, inter = 512, 8, 2, 1024
+    L = Layer(H, nq, nkv, inter, 40)
+    bt = torch.randperm(40, generator=gen(1))[:36].view(3, 12).int().cuda()
+    g = gen(2)
+    ctx = [0, 0, 0]
+    for chunks in ([150, 1, 64], [65, 300, 7], [1, 1, 1], [1, 1, 1], [1, 1, 1]):
+        ctx = [c + n for c, n in zip(ctx, chunks)]
+        meta, starts, pos, slots = layer_meta(chunks, ctx, bt, nq, nkv)
+        T = sum(chunks)
+        x, r = randn(g, T, H, dtype=BF, device="cuda"), randn(g, T, H, dtype=BF, device="cuda")
+        r1 = (x.float() + r.float()).to(BF)
+        k = L.step(x, r, pos, slots, meta)
+        h = r1.double()
+        check_rows(*k["y"], h * L.n1.double() / (h.square().mean(-1, keepdim=True) + 1e-5).sqrt(), 2.0 ** -22, 2.0 ** -17)
+        check_product(k["qkv0"], *k["y"], *L.wqkv, None)
+        check_attention(k["a"], k["qkv"], L.cache, meta, starts, ctx, nq, nkv, L.scale)
+        at = slots.long()
+        v = k["qkv0"][:, (nq + nkv) * D:].view(T, nkv, D)
+        for j in range(nkv):
+            check_rows(L.cache.v[at // 64, j, :, at % 64], L.cache.v_scale[at // 64, j, at % 64], v[:, j], 2.0 ** -24)
+        check_rows(*k["qa"], k["a"], 2.0 ** -24)
+        check_product(k["o"], *k["qa"], *L.wo, None)
+        h = (k["o"].float() + r1.float()).to(BF)
+        assert torch.equal(r, h)
+        h = h.double()
+        check_rows(*k["z"], h * L.n2.double() / (h.square().mean(-1, keepdim=True) + 1e-5).sqrt(), 2.0 ** -22, 2.0 ** -17)
+        check_product(k["gu"], *k["z"], *L.wgu, None)
+        a, b = k["gu"].double().chunk(2, -1)
+        check_rows(*k["act"], a * torch.sigmoid(a) * b, 2.0 ** -18)
+        check_product(k["out"], *k["act"], *L.wdown, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("chunks", [[1, 1, 1], [130, 1, 260]])
+def test_a_captured_layer_replays_what_the_eager_one_computes(chunks):
+    H, nq, nkv, inter = 512, 8, 2, 1024
+    L = Layer(H, nq, nkv, inter, 40)
+    bt = torch.randperm(40, generator=gen(1))[:36].view(3, 12).int().cuda()
+    ctx = [n + 300 for n in chunks]
+    meta, starts, pos, slots = layer_meta(chunks, ctx, bt, nq, nkv)
+    g = gen(4)
+    noise(L.cache)
+    x, r = (torch.zeros(sum(chunks), H, dtype=BF, device="cuda") for _ in range(2))
+    L.step(x, r, pos, slots, meta)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = L.step(x, r, pos, slots, meta)
+    for _ in range(4):
+        x0, r0 = randn(g, *x.shape, dtype=BF, device="cuda"), randn(g, *x.shape, dtype=BF, device="cuda")
+        re = r0.clone()
+        want = L.step(x0, re, pos, slots, meta)["out"].clone()
+        cache = [t.clone() for t in (L.cache.k, L.cache.v, L.cache.k_scale, L.cache.v_scale)]
+        at = slots.long()
+        x.copy_(x0)
+        r.copy_(r0)
+        L.cache.k_scale[at // 64, :, at % 64] = 0
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(kept["out"], want) and torch.equal(r, re)
+        assert all(torch.equal(a, b) for a, b in zip(cache, (L.cache.k, L.cache.v, L.cache.k_scale, L.cache.v_scale)))
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    cases = [product_case("cuda", m, 1100, 1040, seed=s) for s, m in enumerate((1, 48, 200, 700))]
+    want = [Q.linear_int8(*c[:4]).clone() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for st, c in zip(streams, cases):
+            with torch.cuda.stream(st):
+                got.append(Q.linear_int8(*c[:4]))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
