@@ -14,168 +14,474 @@ struct GemmArgs {
   void* y;
   long ldx, ldw, ldy;
   int M, N, K, f32;
+  int splits;    // runs of K; with more than one, int32 sums go to `part` (any order of adding gives the same): [splits][M][ldp],
+  int* part;     // of 256 x 256 tiles [tile - whole][splits][256][256]
+  long ldp;      // a multiple of 8, at least N
+  int whole;     // 256 x 256: tiles in front whose K is not cut
 };
+__device__ const i32x4 kZeros = {0, 0, 0, 0};
 
-// four neighbouring outputs of row m from column n on
-__device__ __forceinline__ void put4(const GemmArgs& a, int m, int n, const i32x4& s) {
-  if (m >= a.M || n >= a.N) return;
-  const float f = a.xs[m];
-  float v[4];
+// R rows by C pieces of V neighbouring columns: row(i) and col(j) are the row and the first column, at(i, j, e) an integer sum.
+// Scales and bias are asked for together, in front of the first store (a load behind a store waits for both).
+template <int R, int C, int V, typename Row, typename Col, typename At>
+__device__ __forceinline__ void put_block(const GemmArgs& a, Row row, Col col, At at) {
+  float f[R], w[C][V], b[C][V] = {};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = min(n + i, a.N - 1);
-    v[i] = (float)s[i] * f * a.ws[c];
-    if (a.bias) v[i] += a.bias[c];
+  for (int i = 0; i < R; ++i) f[i] = a.xs[min(row(i), a.M - 1)];
+#pragma unroll
+  for (int j = 0; j < C; ++j)
+#pragma unroll
+    for (int e = 0; e < V; ++e) w[j][e] = a.ws[min(col(j) + e, a.N - 1)];
+  if (a.bias) {
+#pragma unroll
+    for (int j = 0; j < C; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e) b[j][e] = a.bias[min(col(j) + e, a.N - 1)];
   }
-  const long at = (long)m * a.ldy + n;
-  const bool whole = n + 4 <= a.N;
+  const bool wide = (a.ldy & (V - 1)) == 0 && ((uintptr_t)a.y & 15) == 0;  // (columns start at multiples of V)
+  auto value = [&](int i, int j, int e) { return fmaf((float)at(i, j, e) * f[i], w[j][e], b[j][e]); };
   if (a.f32) {
-    float* const o = (float*)a.y + at;
-    if (whole && ((uintptr_t)o & 15) == 0) {
-      *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
-      return;
-    }
-    for (int i = 0; i < 4 && n + i < a.N; ++i) o[i] = v[i];
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        const int m = row(i), n = col(j);
+        if (m >= a.M) continue;
+        float* const o = (float*)a.y + (long)m * a.ldy + n;
+        if (wide && n + V <= a.N) {
+#pragma unroll
+          for (int e = 0; e < V; e += 4)
+            *reinterpret_cast<f32x4*>(o + e) = f32x4{value(i, j, e), value(i, j, e + 1), value(i, j, e + 2), value(i, j, e + 3)};
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (n + e < a.N) o[e] = value(i, j, e);
+        }
+      }
   } else {
-    uint16_t* const o = (uint16_t*)a.y + at;
-    if (whole && ((uintptr_t)o & 7) == 0) {
-      *reinterpret_cast<u16x4*>(o) = u16x4{f2bf(v[0]), f2bf(v[1]), f2bf(v[2]), f2bf(v[3])};
-      return;
-    }
-    for (int i = 0; i < 4 && n + i < a.N; ++i) o[i] = f2bf(v[i]);
+    typedef uint16_t out_t __attribute__((ext_vector_type(V)));
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        const int m = row(i), n = col(j);
+        if (m >= a.M) continue;
+        uint16_t* const o = (uint16_t*)a.y + (long)m * a.ldy + n;
+        out_t v;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = f2bf(value(i, j, e));
+        if (wide && n + V <= a.N) {
+          *reinterpret_cast<out_t*>(o) = v;
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (n + e < a.N) o[e] = v[e];
+        }
+      }
   }
+}
+__device__ __forceinline__ void put4(const GemmArgs& a, int m, int n, const i32x4& s) {
+  put_block<1, 1, 4>(a, [&](int) { return m; }, [&](int) { return n; }, [&](int, int, int e) { return s[e]; });
 }
 
 // ------------------------------------------------------------ few rows: the weight streams by
-// A workgroup has 16 columns and up to 16 MF rows; its eight waves cut K into eight runs and meet in LDS.
+// A workgroup has 16 columns and up to 16 rows; its eight waves cut K into eight runs and meet in LDS.
 constexpr int kWaves = 8;
-template <int MF>
 __global__ void __launch_bounds__(64 * kWaves) few_kernel(GemmArgs a) {
-  __shared__ i32x4 red[kWaves][MF][64];
+  __shared__ i32x4 red[kWaves][64];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MF;
+  const int n0 = blockIdx.x * 16;
   const uint8_t* const w = a.w + (size_t)min(n0 + r, a.N - 1) * a.ldw;
-  const uint8_t* x[MF];
-#pragma unroll
-  for (int f = 0; f < MF; ++f) x[f] = a.x + (size_t)min(m0 + 16 * f + r, a.M - 1) * a.ldx;
-  const int steps = (a.K + 63) >> 6, per = (steps + kWaves - 1) / kWaves;
-  const int s1 = min(steps, (wv + 1) * per);
-  i32x4 acc[MF] = {};
-  constexpr int U = MF <= 2 ? 4 : 2;
+  const uint8_t* const x = a.x + (size_t)min(r, a.M - 1) * a.ldx;
+  const int steps = (a.K + 63) >> 6, per = (steps + kWaves - 1) / kWaves, s1 = min(steps, (wv + 1) * per);
+  i32x4 acc = {0, 0, 0, 0};
+  constexpr int U = 4;
   for (int s = wv * per; s < s1; s += U) {
-    i32x4 wf[U], xf[U][MF];
+    i32x4 wf[U], xf[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       // a piece behind the row's end: the row's last one is read again, and zeros of x take it out
       const int k = 64 * (s + u) + 16 * g;
       const bool in = s + u < s1 && k < a.K;
       const int kc = in ? k : a.K - 16;
-      wf[u] = ldw_nt<i32x4>(w + kc);
-#pragma unroll
-      for (int f = 0; f < MF; ++f) {
-        xf[u][f] = *reinterpret_cast<const i32x4*>(x[f] + kc);
-        if (!in) xf[u][f] = i32x4{0, 0, 0, 0};
-      }
+      wf[u] = *reinterpret_cast<const i32x4*>(w + kc);
+      xf[u] = *reinterpret_cast<const i32x4*>(x + kc);
+      if (!in) xf[u] = i32x4{0, 0, 0, 0};
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int f = 0; f < MF; ++f) acc[f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u], xf[u][f], acc[f], 0, 0, 0);
+    for (int u = 0; u < U; ++u) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u], xf[u], acc, 0, 0, 0);
   }
-#pragma unroll
-  for (int f = 0; f < MF; ++f) red[wv][f][lane] = acc[f];
+  red[wv][lane] = acc;
   __syncthreads();
-  for (int i = threadIdx.x; i < 64 * MF; i += 64 * kWaves) {
-    const int f = i >> 6, l = i & 63;
-    i32x4 s = red[0][f][l];
+  if (wv) return;
 #pragma unroll
-    for (int k = 1; k < kWaves; ++k) s += red[k][f][l];
-    put4(a, m0 + 16 * f + (l & 15), n0 + 4 * (l >> 4), s);
-  }
+  for (int k = 1; k < kWaves; ++k) acc += red[k][lane];
+  put4(a, r, n0 + 4 * g, acc);
 }
 
-// ------------------------------------------------------------ tiles of 128 x 128
-// Four waves of 64 x 64 each; K in steps of 128 bytes, two stages in LDS (2 x 32 KB) filled through registers.
-constexpr int TB = 128, PITCH = 128 + 16;
-__global__ void __launch_bounds__(256, 2) tile_kernel(GemmArgs a) {
-  __shared__ __attribute__((aligned(16))) uint8_t sm[2][2][TB * PITCH];
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+// ------------------------------------------------------------ staging through LDS
+// A stage holds rows of 128 bytes of K: 16-byte piece c of row r at c ^ ((r >> 1) & 7), so that the 16 lanes of a fragment's
+// read hit 16 different bank groups.  The DMA writes LDS in lane order, so that the exchange is in its source address.
+typedef __attribute__((address_space(3))) void lds_t;
+__device__ __forceinline__ void dma16(const uint8_t* src, uint8_t* dst) { __builtin_amdgcn_global_load_lds(src, (lds_t*)dst, 16, 0, 0); }
+__device__ __forceinline__ void bar() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
+template <int N>
+using ic = std::integral_constant<int, N>;
+
+// Workgroup b of n, such that the workgroups of one XCD (every eighth) have neighbouring numbers.
+__device__ __forceinline__ int near_number(int b, int n) {
+  const int xcd = b & 7, q = n >> 3, r = n & 7;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (b >> 3);
+}
+// Tile t of n_mt x n_nt, in groups of 4 tiles of M by all of N.
+__device__ __forceinline__ void tile_at(int t, int n_mt, int n_nt, int& tm, int& tn) {
+  const int per = 4 * n_nt, first = t / per * 4, gm = min(n_mt - first, 4), u = t % per;
+  tm = first + u % gm;
+  tn = u / gm;
+}
+__device__ __forceinline__ void put_part(const GemmArgs& a, int slice, int m, int n, const i32x4& v) {
+  if (m < a.M && n < a.N) *reinterpret_cast<i32x4*>(a.part + ((size_t)slice * a.M + m) * a.ldp + n) = v;
+}
+
+// ------------------------------------------------------------ middle sizes: tiles of BM x BN behind a ring of stages
+// Waves 2 x WN; NB stages of 128 bytes of K, NB - 1 of them on their way while one is multiplied; one barrier a stage.
+template <int BM, int BN, int NB, int WN>
+__global__ void __launch_bounds__(128 * WN, 2) ring_kernel(GemmArgs a, int n_mt, int n_nt) {
+  constexpr int STAGE = (BM + BN) * 128, I = (BM + BN) / (16 * WN);  // DMAs a wave and stage
+  constexpr int FM = BM / 32, FN = BN / (16 * WN);
+  __shared__ __attribute__((aligned(1024))) uint8_t sm[NB * STAGE];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t0 = near_number(blockIdx.x, n_mt * n_nt * a.splits), slice = t0 % a.splits;
+  int tm, tn;
+  tile_at(t0 / a.splits, n_mt, n_nt, tm, tn);
+  const int m0 = tm * BM, n0 = tn * BN;
+  const int all = (a.K + 127) >> 7, per = (all + a.splits - 1) / a.splits, kt0 = slice * per, nt = min(all - kt0, per);
+
+  const uint8_t* src[I];
+  int lch[I];
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    const int R = 8 * (I * wv + i) + (lane >> 3);  // row of the stage: x's, then w's
+    lch[i] = 16 * ((lane & 7) ^ ((R >> 1) & 7));
+    src[i] = R < BM ? a.x + (size_t)min(m0 + R, a.M - 1) * a.ldx : a.w + (size_t)min(n0 + R - BM, a.N - 1) * a.ldw;
+  }
+  auto issue = [&](int stage, int kt) {
+    const int k = 128 * (kt0 + kt);
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      // (zeros behind K: in both operands, since both may be rows of one tensor that goes on)
+      const uint8_t* p = k + lch[i] < a.K ? src[i] + k + lch[i] : reinterpret_cast<const uint8_t*>(&kZeros);
+      dma16(p, sm + stage * STAGE + (I * wv + i) * 1024);
+    }
+  };
   const int r = lane & 15, g = lane >> 4;
-  const int m0 = blockIdx.y * TB, n0 = blockIdx.x * TB;
-  const int wm = 64 * (wv >> 1), wn = 64 * (wv & 1);
-  i32x4 rx[4], rw[4];
-  const int c = tid & 7, row = tid >> 3;  // 16-byte piece c of rows row, row + 32 ..
-  auto load = [&](int kt) {
-    const int k = 128 * kt + 16 * c;
-    const bool in = k < a.K;
+  const int f0 = r * 128 + 16 * (g ^ ((r >> 1) & 7));
+  const int wr = wv / WN, wc = wv % WN;
+  const int xo = wr * (BM / 2) * 128 + f0, wo = (BM + wc * (BN / WN)) * 128 + f0;
+  i32x4 acc[FM][FN] = {};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int rr = row + 32 * i;
-      rx[i] = rw[i] = i32x4{0, 0, 0, 0};
-      if (in) {
-        rx[i] = *reinterpret_cast<const i32x4*>(a.x + (size_t)min(m0 + rr, a.M - 1) * a.ldx + k);
-        rw[i] = *reinterpret_cast<const i32x4*>(a.w + (size_t)min(n0 + rr, a.N - 1) * a.ldw + k);
-      }
-    }
-  };
-  auto keep = [&](int b) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      *reinterpret_cast<i32x4*>(&sm[b][0][(row + 32 * i) * PITCH + 16 * c]) = rx[i];
-      *reinterpret_cast<i32x4*>(&sm[b][1][(row + 32 * i) * PITCH + 16 * c]) = rw[i];
-    }
-  };
-  i32x4 acc[4][4] = {};
-  const int nt = (a.K + 127) >> 7;
-  load(0);
-  keep(0);
-  for (int kt = 0; kt < nt; ++kt) {
-    __syncthreads();
-    if (kt + 1 < nt) load(kt + 1);
-    const int b = kt & 1;
+  for (int j = 0; j < NB - 1; ++j) issue(j, min(j, nt - 1));
+  for (int i = 0; i < nt; ++i) {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 2) * I) : "memory");
+    bar();
+    issue((i + NB - 1) % NB, min(i + NB - 1, nt - 1));
+    const uint8_t* s = sm + (i % NB) * STAGE;
+    i32x4 xf[2][FM], wf[2][FN];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      i32x4 wf[4], xf[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        xf[i] = *reinterpret_cast<const i32x4*>(&sm[b][0][(wm + 16 * i + r) * PITCH + 64 * ks + 16 * g]);
-        wf[i] = *reinterpret_cast<const i32x4*>(&sm[b][1][(wn + 16 * i + r) * PITCH + 64 * ks + 16 * g]);
-      }
+      for (int f = 0; f < FN; ++f) wf[ks][f] = *reinterpret_cast<const i32x4*>(s + ((wo + 2048 * f) ^ (64 * ks)));
+#pragma unroll
+      for (int f = 0; f < FM; ++f) xf[ks][f] = *reinterpret_cast<const i32x4*>(s + ((xo + 2048 * f) ^ (64 * ks)));
+    }
+    __builtin_amdgcn_sched_barrier(0);  // every read is asked for before the first product
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int f = 0; f < FM; ++f)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[f][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[ks][j], xf[ks][f], acc[f][j], 0, 0, 0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA outlives the workgroup's LDS
+  auto row = [&](int f) { return m0 + wr * (BM / 2) + 16 * f + r; };
+  auto col = [&](int j) { return n0 + wc * (BN / WN) + 16 * j + 4 * g; };
+  if (a.splits > 1) {
+#pragma unroll
+    for (int f = 0; f < FM; ++f)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) put_part(a, slice, row(f), col(j), acc[f][j]);
+    return;
+  }
+  put_block<FM, FN, 4>(a, row, col, [&](int f, int j, int e) { return acc[f][j][e]; });
+}
+
+// ------------------------------------------------------------ large: tiles of 256 x 256, eight phases for two stages
+// Eight waves, 2 x 4, on one compute unit.  A stage of 128 bytes of K is four half tiles (x rows 0-127 and 128-255, w rows
+// likewise) of 16 KB, two stages in LDS.  A stage's product has four phases, one a quadrant of 128 x 128: a phase reads its new
+// fragments (8 of x or 4 of w), asks for one half tile of a later stage, and issues 16 matrix instructions; every fragment is
+// read once a stage.  Waves 4-7 run one barrier behind waves 0-3, so that on each SIMD one wave multiplies while the other
+// reads.  A half tile is asked for two phases after its place was last read and waited for (four half tiles later still on
+// their way) one phase before it is read.  Rows of w are staged so that a lane's two fragments are eight neighbouring columns.
+constexpr int HALF = 128 * 128, BUF = 4 * HALF, OX0 = 0, OX1 = HALF, OW0 = 2 * HALF, OW1 = 3 * HALF;
+__global__ void __launch_bounds__(512, 1) big_kernel(GemmArgs a, int n_mt, int n_nt) {
+  __shared__ __attribute__((aligned(1024))) uint8_t sm[2 * BUF];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wv >> 2, wc = wv & 3;
+  const int b = blockIdx.x;
+  const bool cut = b >= a.whole && a.splits > 1;
+  const int u0 = near_number(b < a.whole ? b : b - a.whole, b < a.whole ? a.whole : gridDim.x - a.whole);
+  const int tile = b < a.whole ? u0 : a.whole + u0 / a.splits, slice = cut ? u0 % a.splits : 0;
+  int tm, tn;
+  tile_at(tile, n_mt, n_nt, tm, tn);
+  const int m0 = tm * 256, n0 = tn * 256;
+  // an even count of stages a run: those behind K are zeros
+  const int all = (a.K + 127) >> 7, runs = cut ? a.splits : 1, nt = ((all + runs - 1) / runs + 1) & ~1, kt0 = slice * nt;
+
+  const uint8_t* const zeros = reinterpret_cast<const uint8_t*>(&kZeros);
+  const uint8_t *xs[2][2], *ws[2][2];
+  int lch[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int R = 16 * wv + 8 * i + (lane >> 3), rho = R & 31;
+    lch[i] = 16 * ((lane & 7) ^ ((R >> 1) & 7));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int n = n0 + 128 * h + (R & ~31) + 8 * ((rho >> 2) & 3) + 4 * (rho >> 4) + (rho & 3);
+      xs[h][i] = a.x + (size_t)min(m0 + 128 * h + R, a.M - 1) * a.ldx + lch[i];
+      ws[h][i] = a.w + (size_t)min(n, a.N - 1) * a.ldw + lch[i];
+    }
+  }
+  auto issue = [&](const uint8_t* const* src, int at, int kt) {
+    const int k = 128 * (kt0 + kt);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) dma16(k + lch[i] < a.K ? src[i] + k : zeros, sm + at + (2 * wv + i) * 1024);
+  };
+  const int r = lane & 15, g = lane >> 4;
+  const int f0 = r * 128 + 16 * (g ^ ((r >> 1) & 7));
+  const int xo = 64 * wr * 128 + f0, wo = 32 * wc * 128 + f0;
+  i32x4 acc[4][4][2] = {};
+  i32x4 xf[4][2], wf0[2][2], wf1[2][2];
+
+  issue(xs[0], OX0, 0);
+  issue(ws[0], OW0, 0);
+  issue(ws[1], OW1, 0);
+  issue(xs[1], OX1, 0);
+  issue(xs[0], BUF + OX0, 1);
+  issue(ws[0], BUF + OW0, 1);
+  asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+  bar();
+  if (wr == 1) bar();
+
+  auto phase = [&](auto PHc, auto Bc, int u) {
+    constexpr int PH = decltype(PHc)::value, B0 = decltype(Bc)::value * BUF, B1 = BUF - B0;
+    auto read_x = [&](int at) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], xf[i], acc[i][j], 0, 0, 0);
+        for (int ks = 0; ks < 2; ++ks) xf[i][ks] = *reinterpret_cast<const i32x4*>(sm + B0 + at + ((xo + 2048 * i) ^ (64 * ks)));
+    };
+    auto read_w = [&](i32x4(&w)[2][2], int at) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) w[j][ks] = *reinterpret_cast<const i32x4*>(sm + B0 + at + ((wo + 2048 * j) ^ (64 * ks)));
+    };
+    if constexpr (PH == 1) {
+      read_w(wf0, OW0);
+      read_x(OX0);
+      issue(ws[1], B1 + OW1, min(u + 1, nt - 1));
+    } else if constexpr (PH == 2) {
+      read_w(wf1, OW1);
+      issue(xs[1], B1 + OX1, min(u + 1, nt - 1));
+    } else if constexpr (PH == 3) {
+      read_x(OX1);
+      issue(xs[0], B0 + OX0, min(u + 2, nt - 1));
+    } else {
+      issue(ws[0], B0 + OW0, min(u + 2, nt - 1));
     }
-    if (kt + 1 < nt) keep(b ^ 1);
+    if constexpr (PH != 3) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    bar();
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const i32x4 w = PH == 1 || PH == 4 ? wf0[j][ks] : wf1[j][ks];
+          acc[PH - 1][i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, xf[i][ks], acc[PH - 1][i][j], 0, 0, 0);
+        }
+    __builtin_amdgcn_s_setprio(0);
+    bar();
+  };
+  for (int u = 0; u < nt; u += 2) {
+    phase(ic<1>{}, ic<0>{}, u);
+    phase(ic<2>{}, ic<0>{}, u);
+    phase(ic<3>{}, ic<0>{}, u);
+    phase(ic<4>{}, ic<0>{}, u);
+    phase(ic<1>{}, ic<1>{}, u + 1);
+    phase(ic<2>{}, ic<1>{}, u + 1);
+    phase(ic<3>{}, ic<1>{}, u + 1);
+    phase(ic<4>{}, ic<1>{}, u + 1);
   }
+  if (wr == 0) bar();
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+
+  // quadrant (x half, w half) is 0 (0,0), 1 (0,1), 2 (1,1), 3 (1,0)
+  auto row = [&](int i) { return m0 + 128 * (i >> 2) + 64 * wr + 16 * (i & 3) + r; };
+  auto col = [&](int j) { return n0 + 128 * j + 32 * wc + 8 * g; };
+  auto quad = [](int i, int j) { return i >= 4 ? 3 - j : j; };
+  if (cut) {
+    int* const p = a.part + ((size_t)(tile - a.whole) * a.splits + slice) * 65536;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) put4(a, m0 + wm + 16 * i + r, n0 + wn + 16 * j + 4 * g, acc[i][j]);
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          *reinterpret_cast<i32x4*>(p + (row(i) - m0) * 256 + col(j) - n0 + 4 * e) = acc[quad(i, j)][i & 3][e];
+    return;
+  }
+  put_block<8, 2, 8>(a, row, col, [&](int i, int j, int e) { return acc[quad(i, j)][i & 3][e >> 2][e & 3]; });
+}
+
+// the runs' sums, scaled: four neighbours a thread
+__global__ void __launch_bounds__(256) join_kernel(GemmArgs a) {
+  const int per = (a.N + 3) >> 2;
+  const long i = blockIdx.x * 256L + threadIdx.x;
+  if (i >= (long)per * a.M) return;
+  const int m = (int)(i / per), n = 4 * (int)(i % per);
+  i32x4 s = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int k = 0; k < a.splits; ++k) s += *reinterpret_cast<const i32x4*>(a.part + ((size_t)k * a.M + m) * a.ldp + n);
+  put4(a, m, n, s);
+}
+
+// the same of the cut tiles of 256 x 256: grid (tiles, 64)
+__global__ void __launch_bounds__(256) join_big_kernel(GemmArgs a, int n_mt, int n_nt) {
+  int tm, tn;
+  tile_at(a.whole + blockIdx.x, n_mt, n_nt, tm, tn);
+  const int row = 4 * blockIdx.y + (threadIdx.x >> 6), c = 4 * (threadIdx.x & 63);
+  if (tm * 256 + row >= a.M || tn * 256 + c >= a.N) return;
+  const int* p = a.part + (size_t)blockIdx.x * a.splits * 65536 + row * 256 + c;
+  i32x4 s = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int k = 0; k < a.splits; ++k) s += *reinterpret_cast<const i32x4*>(p + (size_t)k * 65536);
+  put4(a, tm * 256 + row, tn * 256 + c, s);
+}
+
+// ------------------------------------------------------------ the choice
+// Rows and columns of a tile by kind.
+constexpr int kEdge[7][2] = {{16, 16}, {32, 64}, {64, 64}, {64, 128}, {128, 64}, {128, 128}, {256, 256}};
+
+// Estimated us of a product.  The tiles' time is rounds over the 256 compute units, each `stages` of 128 bytes of K and a fixed part;
+// the middle tiles lie two on a unit, where a stage takes longer.  A product takes no less than its weight's way from memory.
+// Few rows: the weight's way and the rows' reads beside it, or the latency of each wave's turns over K (four steps of 64 bytes
+// a turn), and what a workgroup costs beside its loads, which shows where K is short.  The constants are a fit to times of every kind
+// and cut at 360 sizes from 1 to 5000 rows, 512 to 128256 columns and K from 512 to 28672, the weights from memory: the choice is
+// 1 % from the best one on average.
+inline double cost(int M, int N, int K, int kind, int splits) {
+  constexpr double kStart = 2.25, kByte = 0.172e-6, kJoin = 2.47, kJoinByte = 0.352e-6;
+  // us a stage alone on a unit, by twos (256 x 256: with few units busy), a round's fixed part
+  constexpr double c[7][3] = {{}, {.216, .425, 1.84}, {.272, .526, 1.64}, {.432, .860, 1.53}, {.472, .760, 1.83}, {.623, .466, 2.43}, {1.55, 1.01, 5.11}};
+  const double bytes = (double)N * K;
+  if (kind == 0) {
+    const double turns = (K + 64 * kWaves * 4 - 1) / (64 * kWaves * 4), stream = bytes * (0.163e-6 + 0.0057e-6 * (M - 1));
+    const double wait = turns * (1.13 + 0.04 * (M - 1));
+    return kStart + (wait > stream ? wait : stream) + 0.0025 * ((N + 15) / 16) * (K > 1024 ? 1024. / K : 1.);
+  }
+  const int stages = (K + 127) / 128, per = (stages + splits - 1) / splits;
+  const long tiles = (long)((M - 1) / kEdge[kind][0] + 1) * ((N - 1) / kEdge[kind][1] + 1);
+  const double a = c[kind][0], b = c[kind][1], e = c[kind][2];
+  double t, joined;
+  if (kind >= 5) {
+    const long whole = kind == 6 ? tiles / 256 : tiles * splits / 256, rest = kind == 6 ? tiles % 256 * splits : tiles * splits % 256;
+    t = whole * ((kind == 6 ? stages : per) * a + e) + (rest ? per * (b + (a - b) * rest / 256.) + e : 0);
+    joined = kind == 6 ? 65536. * rest : (double)splits * M * N;
+  } else {
+    const long whole = tiles * splits / 512, rest = tiles * splits % 512;
+    t = whole * (per * b + e) + (rest ? per * (rest > 256 ? b : a) + e : 0);
+    joined = (double)splits * M * N;
+  }
+  if (t < bytes * kByte + 2 * e) t = bytes * kByte + 2 * e;
+  return kStart + t + (splits > 1 ? kJoin + kJoinByte * 4 * joined : 0);
+}
+// Whether `splits` runs of K are possible: none of them empty, and of 256 x 256 tiles only as many as the rest of a round holds.
+inline bool can_cut(int M, int N, int K, int kind, int splits) {
+  if (splits == 1) return true;
+  const int stages = (K + 127) / 128, per = (stages + splits - 1) / splits;
+  if (kind == 0 || (splits - 1) * per >= stages) return false;
+  const long tiles = (long)((M - 1) / kEdge[kind][0] + 1) * ((N - 1) / kEdge[kind][1] + 1);
+  return kind == 6 ? tiles % 256 && tiles % 256 * splits <= 256 : tiles * splits <= 2048;
+}
+
+template <int BM, int BN, int NB, int WN>
+void ring(const GemmArgs& a, hipStream_t st) {
+  const int n_mt = (a.M + BM - 1) / BM, n_nt = (a.N + BN - 1) / BN;
+  hipLaunchKernelGGL((ring_kernel<BM, BN, NB, WN>), dim3(n_mt * n_nt * a.splits), dim3(128 * WN), 0, st, a, n_mt, n_nt);
 }
 
 }  // namespace q8
 }  // namespace k8s
 
-// x [M][ldx], w [N][ldw] int8, 16-byte aligned rows, K % 16 == 0; y bf16, or fp32 with f32.
+// The kernel (kind) and cut of K for these sizes: kind | runs << 8.
+K8S_API int k8s_int8_gemm_plan(int M, int N, int K) {
+  using namespace k8s::q8;
+  static const int runs[] = {1, 2, 3, 4, 6, 8, 12, 16};
+  if (M <= 0 || N <= 0 || K <= 0) return 1 << 8;
+  double best = 0;
+  int plan = 0;
+  for (int kind = M <= 16 ? 0 : 1; kind < 7; ++kind)
+    for (int s : runs) {
+      if (!can_cut(M, N, K, kind, s)) continue;
+      const double t = cost(M, N, K, kind, s);
+      if (!plan || t < best) best = t, plan = kind | s << 8;
+    }
+  return plan;
+}
+
+// int32 numbers of workspace that the plan needs
+K8S_API long k8s_int8_gemm_part(int M, int N, int kind, int splits) {
+  using namespace k8s::q8;
+  if (splits <= 1 || kind < 0 || kind > 6) return 0;
+  const long tiles = (long)((M - 1) / kEdge[kind][0] + 1) * ((N - 1) / kEdge[kind][1] + 1);
+  return kind == 6 ? tiles % 256 * splits * 65536L : (long)splits * M * ((N + 7) / 8 * 8);
+}
+
+// x [M][ldx], w [N][ldw] int8, 16-byte aligned rows, K % 16 == 0; y bf16, or fp32 with f32.  kind: 0 few rows (M <= 16), then tiles
+// of kEdge; those take K in `splits` runs of at least a stage, which leave their sums in `part` (k8s_int8_gemm_part numbers).
 K8S_API int k8s_int8_gemm(const void* x, long ldx, const float* xs, const void* w, long ldw, const float* ws, const float* bias, void* y,
-                          long ldy, int f32, int M, int N, int K, void* stream) {
+                          long ldy, int f32, int M, int N, int K, int kind, int splits, void* part, long parts, void* stream) {
   using namespace k8s::q8;
   if (M <= 0 || N <= 0) return 0;
-  if (K <= 0 || (K & 15) || K > 131056) return (int)hipErrorInvalidValue;
-  const GemmArgs a{(const uint8_t*)x, (const uint8_t*)w, xs, ws, bias, y, ldx, ldw, ldy, M, N, K, f32};
+  if (kind < 0 || kind > 6 || (kind == 0 && M > 16) || K <= 0 || (K & 15) || K > 131056 || splits < 1) return (int)hipErrorInvalidValue;
+  if (!can_cut(M, N, K, kind, splits) || (splits > 1 && (!part || parts < k8s_int8_gemm_part(M, N, kind, splits)))) return (int)hipErrorInvalidValue;
+  const int n_mt = (M - 1) / kEdge[kind][0] + 1, n_nt = (N - 1) / kEdge[kind][1] + 1;
+  if ((long)n_mt * n_nt * splits > 0x7fffffffL || ((long)((N + 3) / 4) * M + 255) / 256 > 0x7fffffffL) return (int)hipErrorInvalidValue;
+  GemmArgs a{(const uint8_t*)x, (const uint8_t*)w, xs, ws, bias, y, ldx, ldw, ldy, M, N, K, f32, splits, (int*)part, (N + 7) / 8 * 8, 0};
   hipStream_t st = (hipStream_t)stream;
-  const dim3 strips((N + 15) / 16);
-  if (M <= 16)
-    hipLaunchKernelGGL(few_kernel<1>, strips, dim3(64 * kWaves), 0, st, a);
-  else if (M <= 32)
-    hipLaunchKernelGGL(few_kernel<2>, strips, dim3(64 * kWaves), 0, st, a);
-  else if (M <= 64)
-    hipLaunchKernelGGL(few_kernel<4>, strips, dim3(64 * kWaves), 0, st, a);
-  else {
-    if ((M + TB - 1) / TB > 65535) return (int)hipErrorInvalidValue;
-    hipLaunchKernelGGL(tile_kernel, dim3((N + TB - 1) / TB, (M + TB - 1) / TB), dim3(256), 0, st, a);
+  switch (kind) {
+    case 0: hipLaunchKernelGGL(few_kernel, dim3(n_nt), dim3(64 * kWaves), 0, st, a); break;
+    case 1: ring<32, 64, 5, 2>(a, st); break;
+    case 2: ring<64, 64, 4, 2>(a, st); break;
+    case 3: ring<64, 128, 3, 4>(a, st); break;
+    case 4: ring<128, 64, 3, 2>(a, st); break;
+    case 5: ring<128, 128, 4, 4>(a, st); break;
+    default: {
+      // the tiles of whole rounds take all of K; those of the last, partial one are cut
+      a.whole = splits > 1 ? n_mt * n_nt / 256 * 256 : n_mt * n_nt;
+      const int rest = n_mt * n_nt - a.whole;
+      hipLaunchKernelGGL(big_kernel, dim3(a.whole + rest * splits), dim3(512), 0, st, a, n_mt, n_nt);
+      if (rest) hipLaunchKernelGGL(join_big_kernel, dim3(rest, 64), dim3(256), 0, st, a, n_mt, n_nt);
+      return (int)hipGetLastError();
+    }
   }
+  if (splits > 1) hipLaunchKernelGGL(join_kernel, dim3((unsigned)(((long)((N + 3) / 4) * M + 255) / 256)), dim3(256), 0, st, a);
   return (int)hipGetLastError();
 }

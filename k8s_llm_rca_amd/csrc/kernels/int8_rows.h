@@ -27,9 +27,14 @@ __device__ __forceinline__ Step row_step(uint32_t top) {
   return {127.f / t, t / 127.f};
 }
 
-// y inv to the nearest integer, in the low byte: 1.5 2^23 puts the integer into the last bits of the sum, which the fma
-// rounds once
-__device__ __forceinline__ uint32_t to_int8(float y, float inv) { return __float_as_uint(fmaf(y, inv, 12582912.f)); }
+// y inv to the nearest integer, ties to even, in the low byte: 1.5 2^23 puts the integer into the last bits of the sum.  The
+// product is rounded first: that brings a tie, which the rounding of inv has moved by less, back to where it is (short
+// numbers are ties often), and gives the plain form's integers.
+__device__ __forceinline__ uint32_t to_int8(float y, float inv) {
+  float p = y * inv;
+  asm("" : "+v"(p));  // (no fma of the two)
+  return __float_as_uint(p + 12582912.f);
+}
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), hi = __builtin_amdgcn_perm(d, c, 0x04000c0cu);
   return lo | hi;

@@ -180,13 +180,15 @@ _SIGS = {
     "k8s_hyper_read": [P, P, I, I, P, P, F, P, I, I, P],
     "k8s_int8_rows": [I, I, P, L, P, P, P, L, P, I, I, F, P],
     "k8s_int8_write": [P, L, P, P, I, P, P, P, P, P, I, I, I, I, L, P],
-    "k8s_int8_gemm": [P, L, P, P, L, P, P, P, L, I, I, I, I, P],
+    "k8s_int8_gemm": [P, L, P, P, L, P, P, P, L, I, I, I, I, I, I, P, L, P],
+    "k8s_int8_gemm_plan": [I, I, I],
+    "k8s_int8_gemm_part": [I, I, I, I],
     "k8s_int8_attn_reply": [P, L, P, P, P, P, I, P, I, P, P, I, I, I, I, F, P, L, P, P, I, I, P, I, P, I, P],
     "k8s_int8_attn_chunk": [P, L, P, P, P, P, I, P, I, P, P, I, I, I, F, P, L, P, P, P, P, P, P, I, I, P, P, P, P, I, P, P, I, P],
     "k8s_walks": [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, P, P, P, P],
 }
 # entry points whose C return type is not int
-_RESTYPES = {"k8s_gemm_big_ws_bytes": ctypes.c_long, "k8s_gemm_big_tail_foreign": ctypes.c_long}
+_RESTYPES = {"k8s_gemm_big_ws_bytes": ctypes.c_long, "k8s_gemm_big_tail_foreign": ctypes.c_long, "k8s_int8_gemm_part": ctypes.c_long}
 
 
 def lib():

@@ -23,6 +23,7 @@ from __future__ import annotations
 import math
 from contextlib import nullcontext
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -37,30 +38,32 @@ MAX_K = 131056
 _ROW_TYPES = (torch.bfloat16, torch.float32)
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
-def _inputs(*tensors) -> None:
+def _inputs(t0: torch.Tensor, *more) -> None:
     """One device for all; none that asks for a gradient."""
-    dev = tensors[0].device
-    for t in tensors:
-        if t is None:
-            continue
-        _need(t.device == dev, f"tensors on {dev} and {t.device}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("the 8-bit operators have no gradients: detach the inputs or call under torch.no_grad()")
+    dev, grad = t0.device, torch.is_grad_enabled()
+    if grad and t0.requires_grad:
+        raise RuntimeError(_NO_GRADIENT)
+    for t in more:
+        if t is not None:
+            if t.device != dev:
+                raise ValueError(f"tensors on {dev} and {t.device}")
+            if grad and t.requires_grad:
+                raise RuntimeError(_NO_GRADIENT)
+
+
+_NO_GRADIENT = "the 8-bit operators have no gradients: detach the inputs or call under torch.no_grad()"
+_HERE = nullcontext()
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _on(t: torch.Tensor):
     """The tensor's device as the current one while a kernel is launched."""
-    return nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE if t.get_device() == _current_device() else torch.cuda.device(t.device)
 
 
 def _aligned(t: torch.Tensor) -> bool:
     """Rows one behind another, each starting at a multiple of 16 bytes."""
-    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or t.stride(0) * t.element_size() % 16 == 0)
+    return t.stride(1) == 1 and t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or t.stride(0) * t.element_size() % 16 == 0)
 
 
 def _ld(t: torch.Tensor) -> int:
@@ -81,28 +84,32 @@ def _quantised(y: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 def _rows(mode: int, x: torch.Tensor, H: int, out, scale, w=None, residual=None, eps: float = 0.0):
     T = x.shape[0]
     _inputs(x, out, scale, w, residual)
-    if x.dtype not in _ROW_TYPES:
-        raise TypeError(f"rows must be bfloat16 or float32, not {x.dtype}")
-    _need(H > 0 and H % 16 == 0, f"rows of a multiple of 16 values, not {H}")
+    dtype = x.dtype
+    if dtype not in _ROW_TYPES:
+        raise TypeError(f"rows must be bfloat16 or float32, not {dtype}")
+    if H <= 0 or H % 16:
+        raise ValueError(f"rows of a multiple of 16 values, not {H}")
     if out is None:
         out = torch.empty((T, H), dtype=torch.int8, device=x.device)
+    elif out.dtype != torch.int8 or out.shape != (T, H) or not _aligned(out):
+        raise ValueError(f"out must be int8 {[T, H]} with 16-byte rows")
     if scale is None:
         scale = torch.empty(T, dtype=torch.float32, device=x.device)
-    _need(out.dtype == torch.int8 and out.shape == (T, H) and _aligned(out), "out must be int8 [T, H] with 16-byte rows")
-    _need(scale.dtype == torch.float32 and scale.shape == (T,) and scale.is_contiguous(), "scale must be contiguous float32 [T]")
-    if w is not None:
-        _need(w.dtype == x.dtype and w.shape == (H,), f"the norm's weight must be {x.dtype} [{H}]")
-    if residual is not None:
-        _need(residual.dtype == x.dtype and residual.shape == x.shape and residual.is_contiguous() and residual.data_ptr() % 16 == 0,
-              "the residual must be contiguous, 16-byte aligned and of the rows' shape and type")
+    elif scale.dtype != torch.float32 or scale.shape != (T,) or not scale.is_contiguous():
+        raise ValueError(f"scale must be contiguous float32 {[T]}")
+    if w is not None and (w.dtype != dtype or w.shape != (H,)):
+        raise ValueError(f"the norm's weight must be {dtype} {[H]}")
+    if residual is not None and (residual.dtype != dtype or residual.shape != x.shape or not residual.is_contiguous()
+                                 or residual.data_ptr() % 16):
+        raise ValueError("the residual must be contiguous, 16-byte aligned and of the rows' shape and type")
     if use_hip(x):
         if not _aligned(x):
             x = x.clone(memory_format=torch.contiguous_format)
         if w is not None and not (w.is_contiguous() and w.data_ptr() % 16 == 0):
             w = w.clone(memory_format=torch.contiguous_format)
         with _on(x):
-            check(lib().k8s_int8_rows(mode, int(x.dtype == torch.float32), ptr(x), _ld(x), ptr(residual), ptr(w), ptr(out), _ld(out),
-                                      ptr(scale), T, H, float(eps), stream_ptr(x)), "int8_rows")
+            check(lib().k8s_int8_rows(mode, dtype == torch.float32, x.data_ptr(), _ld(x), ptr(residual), ptr(w), out.data_ptr(), _ld(out),
+                                      scale.data_ptr(), T, H, eps, stream_ptr(x)), "int8_rows")
         return out, scale
     y = x.float()
     if mode == 1:
@@ -122,7 +129,8 @@ def _rows(mode: int, x: torch.Tensor, H: int, out, scale, w=None, residual=None,
 def quantize_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None,
                   scale: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """``x`` [T, H] (bf16 or fp32) as int8 rows and fp32 scales [T].  Of a weight [N, K]: its output channels."""
-    _need(x.dim() == 2, "rows must be a matrix")
+    if x.dim() != 2:
+        raise ValueError("rows must be a matrix")
     return _rows(0, x, x.shape[1], out, scale)
 
 
@@ -130,7 +138,8 @@ def silu_mul_int8(gu: torch.Tensor, out: Optional[torch.Tensor] = None,
                   scale: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """``silu(gate) * up`` of ``gu`` [T, 2 I] (gate columns first), as ``norm.silu_mul``, in int8 rows: the product is
     quantised from fp32 and never written in a wider type."""
-    _need(gu.dim() == 2 and gu.shape[1] % 2 == 0, "gate and up columns side by side in a matrix")
+    if gu.dim() != 2 or gu.shape[1] % 2:
+        raise ValueError("gate and up columns side by side in a matrix")
     return _rows(1, gu, gu.shape[1] // 2, out, scale)
 
 
@@ -138,38 +147,58 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Op
                  out: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """``rmsnorm(x + residual) * weight`` in int8 rows; ``residual`` is updated in place to ``x + residual``, rounded to its
     type, and the norm is that of the rounded sum (as ``norm.rmsnorm``)."""
-    _need(x.dim() == 2, "rows must be a matrix")
+    if x.dim() != 2:
+        raise ValueError("rows must be a matrix")
     return _rows(2, x, x.shape[1], out, scale, weight, residual, eps)
 
 
 # ------------------------------------------------------------------ products
+FEW, T32, T64, T64_128, T128_64, T128, T256 = range(7)
+
+
+@lru_cache(maxsize=4096)
+def product_plan(M: int, N: int, K: int) -> Tuple[int, int, int]:
+    """(kernel, runs of K, int32 numbers of workspace) of a product: the cheapest by the cost model beside the kernels."""
+    p = lib().k8s_int8_gemm_plan(M, N, K)
+    kind, runs = p & 255, p >> 8
+    return kind, runs, lib().k8s_int8_gemm_part(M, N, kind, runs)
+
+
 def linear_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
                 out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``(x @ w.T) * x_scale[:, None] * w_scale (+ bias)`` for int8 ``x`` [M, K] and ``w`` [N, K], scales fp32 [M] and [N],
     ``bias`` fp32 [N]; bf16 or fp32 out.  The integer sum is exact, so a row's result does not depend on the rows beside it."""
-    _need(x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1], "x [M, K] and w [N, K]")
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"x [M, K] and w [N, K], not {list(x.shape)} and {list(w.shape)}")
     M, K = x.shape
     N = w.shape[0]
     _inputs(x, x_scale, w, w_scale, bias, out)
     if x.dtype != torch.int8 or w.dtype != torch.int8:
         raise TypeError(f"x and w must be int8, not {x.dtype} and {w.dtype}")
-    _need(0 < K <= MAX_K and K % 16 == 0, f"K must be a multiple of 16 up to {MAX_K}, not {K}")
-    for t, n, name in ((x_scale, M, "x_scale"), (w_scale, N, "w_scale"), (bias, N, "bias")):
-        _need(t is None or (t.dtype == torch.float32 and t.shape == (n,) and t.is_contiguous()), f"{name} must be contiguous float32 [{n}]")
+    if not 0 < K <= MAX_K or K % 16:
+        raise ValueError(f"K must be a multiple of 16 up to {MAX_K}, not {K}")
+    for t, n in ((x_scale, M), (w_scale, N), (bias, N)):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous()):
+            raise ValueError(f"x_scale {[M]}, w_scale {[N]} and bias {[N]} must be contiguous float32, not {t.dtype} {list(t.shape)}")
     if out is None:
         if out_dtype not in _ROW_TYPES:
             raise TypeError(f"out_dtype must be bfloat16 or float32, not {out_dtype}")
         out = torch.empty((M, N), dtype=out_dtype, device=x.device)
-    _need(out.dtype in _ROW_TYPES and out.shape == (M, N) and out.stride(1) == 1, "out must be bfloat16 or float32 [M, N], its rows dense")
+    elif out.dtype not in _ROW_TYPES or out.shape != (M, N) or out.stride(1) != 1:
+        raise ValueError(f"out must be bfloat16 or float32 {[M, N]}, its rows dense")
     if M == 0 or N == 0:
         return out
     if use_hip(x):
         if not _aligned(x):
             x = x.clone(memory_format=torch.contiguous_format)
-        _need(_aligned(w), "w's rows must be dense and start at multiples of 16 bytes")
+        if not _aligned(w):
+            raise ValueError("w's rows must be dense and start at multiples of 16 bytes")
+        kind, runs, n = product_plan(M, N, K)
         with _on(x):
-            check(lib().k8s_int8_gemm(ptr(x), _ld(x), ptr(x_scale), ptr(w), _ld(w), ptr(w_scale), ptr(bias), ptr(out), _ld(out),
-                                      int(out.dtype == torch.float32), M, N, K, stream_ptr(x)), "int8_gemm")
+            part = torch.empty(n, dtype=torch.int32, device=x.device) if n else None
+            check(lib().k8s_int8_gemm(x.data_ptr(), _ld(x), x_scale.data_ptr(), w.data_ptr(), _ld(w), w_scale.data_ptr(), ptr(bias),
+                                      out.data_ptr(), _ld(out), out.dtype == torch.float32, M, N, K, kind, runs, ptr(part), n,
+                                      stream_ptr(x)), "int8_gemm")
         return out
     # (in fp64 every partial sum is an integer below 2^53: exact)
     y = (x.double() @ w.double().T).float() * x_scale[:, None] * w_scale
@@ -190,14 +219,16 @@ class Int8KV:
 
     def __post_init__(self):
         NB, nkv, BS, D = self.k.shape
-        _need(D == HEAD_DIM and self.v.shape == (NB, nkv, D, BS), "k must be [NB, nkv, BS, 128] and v [NB, nkv, 128, BS]")
-        _need(BS > 0 and BS % 64 == 0, f"pages of a multiple of 64 tokens, not {BS}")
-        _need(self.k.dtype == torch.int8 == self.v.dtype, "k and v must be int8")
-        for s in (self.k_scale, self.v_scale):
-            _need(s.dtype == torch.float32 and s.shape == (NB, nkv, BS), "scales must be float32 [NB, nkv, BS]")
-        for t in (self.k, self.v, self.k_scale, self.v_scale):
-            _need(t.is_contiguous() and t.data_ptr() % 16 == 0 and t.device == self.k.device,
-                  "the cache's tensors must be contiguous, 16-byte aligned and on one device")
+        if D != HEAD_DIM or self.v.shape != (NB, nkv, D, BS):
+            raise ValueError("k must be [NB, nkv, BS, 128] and v [NB, nkv, 128, BS]")
+        if BS <= 0 or BS % 64:
+            raise ValueError(f"pages of a multiple of 64 tokens, not {BS}")
+        if self.k.dtype != torch.int8 or self.v.dtype != torch.int8:
+            raise ValueError("k and v must be int8")
+        if any(s.dtype != torch.float32 or s.shape != (NB, nkv, BS) for s in (self.k_scale, self.v_scale)):
+            raise ValueError("scales must be float32 [NB, nkv, BS]")
+        if any(not t.is_contiguous() or t.data_ptr() % 16 or t.device != self.k.device for t in (self.k, self.v, self.k_scale, self.v_scale)):
+            raise ValueError("the cache's tensors must be contiguous, 16-byte aligned and on one device")
 
     @staticmethod
     def empty(num_blocks: int, nkv: int, block_size: int, device) -> "Int8KV":
@@ -208,17 +239,14 @@ class Int8KV:
 
 
 def _heads(rows: torch.Tensor, cache: Int8KV, nq: int, nkv: int, width: int, what: str) -> None:
-    _inputs(rows, cache.k)
-    _need(nkv > 0 and nq > 0 and nq % nkv == 0, f"{nq} query heads over {nkv} key heads")
-    _need(cache.k.shape[1] == nkv, f"a cache of {cache.k.shape[1]} heads, not {nkv}")
-    _need(rows.dim() == 2 and rows.shape[1] >= width, f"{what} needs {width} columns")
+    if nkv <= 0 or nq <= 0 or nq % nkv:
+        raise ValueError(f"{nq} query heads over {nkv} key heads")
+    if cache.k.shape[1] != nkv:
+        raise ValueError(f"a cache of {cache.k.shape[1]} heads, not {nkv}")
+    if rows.dim() != 2 or rows.shape[1] < width:
+        raise ValueError(f"{what} needs {width} columns")
     if rows.is_cuda and rows.dtype != torch.bfloat16:
         raise TypeError(f"{what} must be bfloat16, not {rows.dtype}")
-
-
-def _ints(*tensors) -> None:
-    for t, shape, name in tensors:
-        _need(t.dtype == torch.int32 and t.is_contiguous() and t.shape == shape, f"{name} must be contiguous int32 {list(shape)}")
 
 
 def rope_kv_write_int8(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, slots: Optional[torch.Tensor], cache: Int8KV,
@@ -229,19 +257,22 @@ def rope_kv_write_int8(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torc
     ``attention.rope_kv_write``, the rows of one call have different slots."""
     T = qkv.shape[0]
     _heads(qkv, cache, nq, nkv, (nq + 2 * nkv) * HEAD_DIM, "qkv")
-    _inputs(qkv, positions, cos_sin, slots)
-    _ints((positions, (T,), "positions"), *([] if slots is None else [(slots, (T,), "slots")]))
-    _need(cos_sin.dtype == torch.float32 and cos_sin.is_contiguous() and cos_sin.dim() == 2 and cos_sin.shape[1] == HEAD_DIM
-          and cos_sin.shape[0] > 0, "cos_sin must be contiguous float32 [positions, 128]")
+    _inputs(qkv, positions, cos_sin, slots, cache.k)
+    for t in (positions, slots):
+        if t is not None and (t.dtype != torch.int32 or t.shape != (T,) or not t.is_contiguous()):
+            raise ValueError(f"positions and slots must be contiguous int32 {[T]}, not {t.dtype} {list(t.shape)}")
+    if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or cos_sin.dim() != 2 or cos_sin.shape[1] != HEAD_DIM or not cos_sin.shape[0]:
+        raise ValueError("cos_sin must be contiguous float32 [positions, 128]")
     NB, _, BS, D = cache.k.shape
     if T == 0:
         return
     if use_hip(qkv):
-        _need(_aligned(qkv) and cos_sin.data_ptr() % 16 == 0, "qkv's rows must be dense and start at multiples of 16 bytes")
+        if not _aligned(qkv) or cos_sin.data_ptr() % 16:
+            raise ValueError("the rows of qkv and cos_sin must be dense and start at multiples of 16 bytes")
         with _on(qkv):
-            check(lib().k8s_int8_write(ptr(qkv), _ld(qkv), ptr(positions), ptr(cos_sin), cos_sin.shape[0], ptr(slots), ptr(cache.k),
-                                       ptr(cache.v), ptr(cache.k_scale), ptr(cache.v_scale), T, nq, nkv, BS, NB * BS, stream_ptr(qkv)),
-                  "int8_write")
+            check(lib().k8s_int8_write(qkv.data_ptr(), _ld(qkv), positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], ptr(slots),
+                                       cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), T, nq, nkv,
+                                       BS, NB * BS, stream_ptr(qkv)), "int8_write")
         return
     nh = nq + nkv
     cos, sin = cos_sin[positions.long().clamp(0, cos_sin.shape[0] - 1)][:, None].chunk(2, -1)
@@ -268,41 +299,49 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
     T = q.shape[0]
     _heads(q, cache, nq, nkv, nq * HEAD_DIM, "q")
     NB, _, BS, D = cache.k.shape
-    S = meta.num_seqs
-    _inputs(q, meta.block_tables, meta.ctx_lens, meta.q_start, out)
+    S, bt, ctx, starts = meta.num_seqs, meta.block_tables, meta.ctx_lens, meta.q_start
+    _inputs(q, bt, ctx, starts, cache.k, out)
     if out is None:
         out = torch.empty((T, nq * D), dtype=q.dtype, device=q.device)
-    _need(out.shape == (T, nq * D) and out.dtype == q.dtype and out.stride(1) == 1, "out must be [T, nq 128] of q's type, its rows dense")
+    elif out.shape != (T, nq * D) or out.dtype != q.dtype or out.stride(1) != 1:
+        raise ValueError("out must be [T, nq 128] of q's type, its rows dense")
     if T == 0 or S == 0:
         return out
     if not use_hip(q):
         return _attention_plain(q, cache, meta, nq, nkv, scale, out)
-    bt = meta.block_tables
-    _need(bt.dtype == torch.int32 and bt.dim() == 2 and bt.shape[0] >= S and bt.stride(1) == 1, "block_tables must be int32 [S, pages]")
-    _need(meta.ctx_lens.dtype == torch.int32 == meta.q_start.dtype and meta.ctx_lens.numel() >= S and meta.q_start.numel() >= S + 1,
-          "ctx_lens must be int32 [S] and q_start int32 [S + 1]")
-    _need(_aligned(q), "q's rows must be dense and start at multiples of 16 bytes")
+    if bt.dtype != torch.int32 or bt.dim() != 2 or bt.shape[0] < S or bt.stride(1) != 1:
+        raise ValueError("block_tables must be int32 [S, pages]")
+    if ctx.dtype != torch.int32 or starts.dtype != torch.int32 or ctx.numel() < S or starts.numel() < S + 1:
+        raise ValueError("ctx_lens must be int32 [S] and q_start int32 [S + 1]")
+    if not _aligned(q):
+        raise ValueError("q's rows must be dense and start at multiples of 16 bytes")
     G, L = nq // nkv, lib()
-    common = (ptr(q), _ld(q), ptr(cache.k), ptr(cache.v), ptr(cache.k_scale), ptr(cache.v_scale), NB, ptr(bt), bt.stride(0) if S > 1 else bt.shape[1],
-              ptr(meta.ctx_lens), ptr(meta.q_start))
+    common = (q.data_ptr(), _ld(q), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), NB,
+              bt.data_ptr(), bt.stride(0) if S > 1 else bt.shape[1], ctx.data_ptr(), starts.data_ptr())
     if meta.decode:
-        _need(T == S, "a reply step has one row a sequence")
-        _need(G <= 16, f"{G} query heads a key head: a reply step takes 16")
-        _need(meta.items is not None and meta.items.dtype == torch.int32, "the step has no plan: attach_decode_plan")
-        _need(meta.n_parts == 1 or meta.part_o is not None, "a plan of several parts needs part_o and part_ml")
+        if T != S:
+            raise ValueError(f"a reply step has one row a sequence, not {T} for {S}")
+        if G > 16:
+            raise ValueError(f"{G} query heads a key head: a reply step takes 16")
+        if meta.items is None or meta.items.dtype != torch.int32:
+            raise ValueError("the step has no plan: attach_decode_plan")
+        if meta.n_parts > 1 and meta.part_o is None:
+            raise ValueError("a plan of several parts needs part_o and part_ml")
         grid = max(1, meta.grid_waves or min(A.DECODE_WAVE_SLOTS, meta.n_items * nkv))
         with _on(q):
-            check(L.k8s_int8_attn_reply(*common, S, nq, nkv, BS, float(scale), ptr(out), _ld(out), ptr(meta.part_o), ptr(meta.part_ml),
-                                        meta.n_parts, meta.part_size, ptr(meta.items), meta.n_items, ptr(meta.d_n_items), grid,
+            check(L.k8s_int8_attn_reply(*common, S, nq, nkv, BS, scale, out.data_ptr(), _ld(out), ptr(meta.part_o), ptr(meta.part_ml),
+                                        meta.n_parts, meta.part_size, meta.items.data_ptr(), meta.n_items, ptr(meta.d_n_items), grid,
                                         stream_ptr(q)), "int8_attn_reply")
         return out
     rows = A.prefill_tile_tokens(G, BS) * G
-    _need(rows <= A.PF8_ROWS, f"{G} query heads a key head: a tile takes {A.PF8_ROWS}")
-    _need(meta.tile_seq is not None and meta.tile_kv1 is not None, "the step has no plan: attach_plan")
+    if rows > A.PF8_ROWS:
+        raise ValueError(f"{G} query heads a key head: a tile takes {A.PF8_ROWS}")
+    if meta.tile_seq is None or meta.tile_kv1 is None:
+        raise ValueError("the step has no plan: attach_plan")
     if meta.n_merge and meta.pf_o is None:
         meta.pf_o, meta.pf_ml = A.prefill_workspace(nkv, q.device, max(meta.m_slot0_end(), 1))
     with _on(q):
-        check(L.k8s_int8_attn_chunk(*common, nq, nkv, BS, float(scale), ptr(out), _ld(out), ptr(meta.tile_seq), ptr(meta.tile_tok0),
+        check(L.k8s_int8_attn_chunk(*common, nq, nkv, BS, scale, out.data_ptr(), _ld(out), ptr(meta.tile_seq), ptr(meta.tile_tok0),
                                     ptr(meta.tile_len), ptr(meta.tile_kv0), ptr(meta.tile_kv1), ptr(meta.tile_slot), meta.n_tiles, rows,
                                     ptr(meta.m_tok0), ptr(meta.m_len), ptr(meta.m_slot0), ptr(meta.m_np), meta.n_merge, ptr(meta.pf_o),
                                     ptr(meta.pf_ml), A.PF8_ROWS, stream_ptr(q)), "int8_attn_chunk")

@@ -141,6 +141,20 @@ def check_product(y, x, xs, w, ws, b):
     assert bool(((y.double() - want).abs() <= tol).all())
 
 
+def forced(monkeypatch, kind, runs):
+    from k8s_llm_rca_amd.ops._lib import lib
+    monkeypatch.setattr(Q, "product_plan", lambda M, N, K: (kind, runs, lib().k8s_int8_gemm_part(M, N, kind, runs)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,runs", [(4352, 4097, 3), (300, 4096 * 16 - 5, 1), (8200, 2040, 5)])
+def test_product_of_more_than_a_round_of_tiles(M, N, runs, monkeypatch):
+    """256 x 256 tiles: whole rounds of 256, the rest's K cut."""
+    forced(monkeypatch, Q.T256, runs)
+    args = product_case("cuda", M, N, 1040, BF, True)
+    check_product(Q.linear_int8(*args[:4], bias=args[4]), *args)
+
+
 SIZES = [(1, 1, 16), (1, 6144, 4096), (2, 17, 48), (5, 33, 80), (16, 64, 64), (17, 100, 1040), (31, 515, 144), (33, 256, 512),
          (48, 1000, 4096), (64, 47, 4112), (65, 129, 256), (100, 300, 2064), (128, 128, 128), (129, 257, 400), (200, 1030, 1024),
          (256, 256, 256), (257, 513, 272), (300, 4096, 512), (513, 1000, 16), (1000, 777, 1152), (1111, 2048, 640), (2050, 300, 2048)]
@@ -152,6 +166,20 @@ SIZES = [(1, 1, 16), (1, 6144, 4096), (2, 17, 48), (5, 33, 80), (16, 64, 64), (1
 def test_product(M, N, K, dtype, bias):
     args = product_case("cuda", M, N, K, dtype, bias)
     check_product(Q.linear_int8(*args[:4], bias=args[4], out_dtype=dtype), *args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(1, 3, 16), (50, 70, 400), (129, 257, 1040), (300, 515, 2064), (64, 128, 128)])
+@pytest.mark.parametrize("kind", [Q.T32, Q.T64, Q.T64_128, Q.T128_64, Q.T128, Q.T256])
+@pytest.mark.parametrize("runs", [1, 2, 3, 8])
+def test_every_kernel_of_a_product(M, N, K, kind, runs, monkeypatch):
+    """Whichever tiles and runs of K the plan would choose."""
+    runs = min(runs, -(-K // 128))
+    runs = -(-(-(-K // 128)) // -(-(-(-K // 128)) // runs))   # (none of them empty)
+    forced(monkeypatch, kind, runs)
+    for dtype in (BF, F32):
+        args = product_case("cuda", M, N, K, dtype, True)
+        check_product(Q.linear_int8(*args[:4], bias=args[4], out_dtype=dtype), *args)
 
 
 @pytest.mark.parametrize("M,N,K", [(1, 1, 16), (3, 5, 48), (33, 17, 4096)])
