@@ -36,7 +36,7 @@ struct AttnArgs {
   int n_parts, part_size;
   // chunks: tiles of rows and runs of 64-key pages
   const int *tile_seq, *tile_tok0, *tile_len, *tile_kv0, *tile_kv1, *tile_slot;
-  int n_tiles, tile_waves;
+  int n_tiles;
   const int *m_tok0, *m_len, *m_slot0, *m_np;
   int n_merge, slot_rows;
 };
@@ -103,8 +103,7 @@ __device__ __forceinline__ void walk(State& st, const AttnArgs& a, const int* bt
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (kb + 16 * g + 4 * t + i >= lim) sc[t][i] = -INFINITY;
-          if (kb + 16 * g + 4 * t + i >= k1) vs[t][i] = 0.f;
+          if (kb + 16 * g + 4 * t + i >= lim) sc[t][i] = -INFINITY, vs[t][i] = 0.f;
         }
     }
     float top = -INFINITY;
@@ -127,8 +126,7 @@ __device__ __forceinline__ void walk(State& st, const AttnArgs& a, const int* bt
       for (int i = 0; i < 4; ++i) {
         const float e = __builtin_amdgcn_exp2f(sc[t][i] - sub);
         sum += e;
-        // (a row's own limit may lie in front of the wave's: its weight there is zero, and so is the product, unless the scale is a NaN)
-        pf[t >> 1][4 * (t & 1) + i] = (__bf16)(sc[t][i] == -INFINITY ? 0.f : e * vs[t][i]);
+        pf[t >> 1][4 * (t & 1) + i] = (__bf16)(e * vs[t][i]);
       }
     st.l = st.l * alpha + sum;
     st.m = m;
@@ -233,32 +231,239 @@ __global__ void __launch_bounds__(D) reply_merge_kernel(AttnArgs a) {
 }
 
 // ------------------------------------------------------------------ chunks
-// grid: tiles * nkv * tile_waves, a wave each
-__global__ void __launch_bounds__(64, 2) chunk_kernel(AttnArgs a) {
-  const int lane = threadIdx.x, r = lane & 15, g = lane >> 4;
-  const int w = blockIdx.x % a.tile_waves, kvh = blockIdx.x / a.tile_waves % a.nkv, tile = blockIdx.x / a.tile_waves / a.nkv;
-  const int seq = a.tile_seq[tile], tok0 = a.tile_tok0[tile], len = a.tile_len[tile], rows = len * a.G;
-  if (16 * w >= rows) return;
+// A workgroup holds up to 256 rows (token, q head) of one kv head, 32 a wave, and walks pages of 64 keys.  Keys and values are made
+// bf16 once for all waves on their way into LDS (two pages each): 16 of each a thread, asked for a page ahead.
+// v_mfma_f32_32x32x16_bf16, S^T = K Q^T: row rho of the 32-key half kt is key 32 kt + 16 (reg >> 3) + 8 hi + (reg & 7) with
+// reg = (rho & 3) + 4 (rho >> 3), hi = (rho >> 2) & 1, so that a lane has one row's keys 16 s + 8 hi .. + 7 in registers
+// 8 s .. 8 s + 7: the second operand of O^T += V^T P^T as they are.
+// LDS: a key's 256 bytes with 16-byte piece c at c ^ (key & 15), a dim's 128 bytes with piece c at c ^ ((dim >> 1) & 7): no bank
+// conflicts in either direction.
+// A turn has page i's softmax beside the products of its neighbours, so that the vector and the matrix units work at once: the
+// weights of its first 32 keys beside V(i - 1), those of the others beside the first half of K(i + 1), whose scores take the
+// registers that the weights have left.
+constexpr int kRows = 256, kPitch = 272;
+struct ChunkLds {
+  uint8_t k[2][64 * 256], v[2][D * 128];
+  float s[4][2][64];  // keys' scales (with the softmax's, in powers of two), values'
+};
+__device__ __forceinline__ void lds_bar() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+__global__ void __launch_bounds__(512, 1) chunk_kernel(AttnArgs a) {
+  __shared__ __attribute__((aligned(1024))) union {
+    ChunkLds p;
+    uint8_t o[8 * 32 * kPitch];
+  } sm;
+  const int kvh = blockIdx.x % a.nkv, tile = blockIdx.x / a.nkv;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 31, hi = lane >> 5;
+  const int seq = a.tile_seq[tile], tok0 = a.tile_tok0[tile], len = a.tile_len[tile], rows = min(len * a.G, kRows);
   const int qs = a.q_start[seq], base = a.ctx[seq] - (a.q_start[seq + 1] - qs) + (tok0 - qs);
-  const int row = 16 * w + r, tt = min(row, rows - 1) / a.G, head = kvh * a.G + min(row, rows - 1) % a.G;
-  const bool valid = row < rows;
-  const int lo = 16 * w / a.G, hi = min(rows - 1, 16 * w + 15) / a.G;
-  const int k0 = a.tile_kv0[tile] * 64, k1 = max(k0, (int)min(min((long)base + hi + 1, a.tile_kv1[tile] * 64L), (long)a.bt_stride * a.BS));
-  State st;
-  load_q(st, a, tok0 + tt, head, valid, g);
-  walk(st, a, a.bt + (size_t)seq * a.bt_stride, kvh, k0, k1, base + lo + 1, base + tt + 1, lane);
-  float m[4], l[4];
-  row_stats(st, g, m, l);
-  const int slot = a.tile_slot[tile];
+  const int* const bt = a.bt + (size_t)seq * a.bt_stride;
+  const int grow = 32 * w + r;
+  const bool valid = grow < rows;
+  const int end = min(base + len, a.bt_stride * a.BS);      // keys of the whole tile
+  const int p0 = a.tile_kv0[tile], np = min(a.tile_kv1[tile], (end + 63) >> 6) - p0;
+  // this lane's row sees keys below `limit`, every row of the wave those below `lo`
+  const int limit = min(valid ? base + grow / a.G + 1 : 0, end), lo = 32 * w + 31 < rows ? base + 32 * w / a.G + 1 : 0;
+
+  bf16x8 qf[8];
+  {
+    const int at = min(grow, rows - 1), tt = at / a.G;
+    const uint16_t* const q = a.q + (long)(tok0 + tt) * a.ldq + (kvh * a.G + at - tt * a.G) * D + 8 * hi;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int rr = 16 * w + 4 * g + i;
-    if (rr >= rows) continue;
-    if (slot < 0) {
-      put_row(st, i, l[i] == 0.f ? 0.f : 1.f / l[i], a.out + (long)(tok0 + rr / a.G) * a.ldo + (kvh * a.G + rr % a.G) * D, r);
+    for (int s = 0; s < 8; ++s) {
+      u16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (valid) z = *reinterpret_cast<const u16x8*>(q + 16 * s);
+      qf[s] = __builtin_bit_cast(bf16x8, z);
+    }
+  }
+  f32x16 o[4] = {};
+  float m = -INFINITY, l = 0.f;
+
+  // staging: 16 dims of key tid >> 3, 16 keys of dim tid >> 2, a key's scales
+  const int key = tid >> 3, kc = tid & 7, dim = tid >> 2, vc = tid & 3;
+  auto page_of = [&](int i, int& off) {
+    const int k0 = 64 * (p0 + min(i, np - 1));
+    off = k0 % a.BS;
+    return (size_t)min(max(__builtin_amdgcn_readfirstlane(bt[k0 / a.BS]), 0), a.NB - 1) * a.nkv + kvh;
+  };
+  u32x4 kx, vx;
+  float ksx = 0.f, vsx = 0.f;
+  auto ask_k = [&](int i) {
+    int off;
+    const size_t page = page_of(i, off);
+    kx = *reinterpret_cast<const u32x4*>(a.k + (page * a.BS + off + key) * D + 16 * kc);
+    if (tid < 64) {
+      ksx = a.ks[page * a.BS + off + tid];
+      vsx = a.vs[page * a.BS + off + tid];
+    }
+  };
+  auto ask_v = [&](int i) {
+    int off;
+    const size_t page = page_of(i, off);
+    vx = *reinterpret_cast<const u32x4*>(a.v + (page * D + dim) * a.BS + off + 16 * vc);
+  };
+  auto keep_k = [&](int i) {
+    uint8_t* const kr = sm.p.k[i & 1] + key * 256;
+    *reinterpret_cast<bf16x8*>(kr + 16 * ((2 * kc) ^ (key & 15))) = to_bf16x8(kx[0], kx[1]);
+    *reinterpret_cast<bf16x8*>(kr + 16 * ((2 * kc + 1) ^ (key & 15))) = to_bf16x8(kx[2], kx[3]);
+    if (tid < 64) {
+      // a key behind the context is nothing, whatever its scales say; a value that is no number makes its key's score none, so
+      // that the weights' factor is always a number (and a hidden key's product zero)
+      const bool in = 64 * (p0 + i) + tid < end, nan = vsx != vsx;
+      sm.p.s[i & 3][0][tid] = in ? (nan ? vsx : ksx * a.scale_log2) : 0.f;
+      sm.p.s[i & 3][1][tid] = in && !nan ? vsx : 0.f;
+    }
+  };
+  auto keep_v = [&](int i) {
+    uint8_t* const vr = sm.p.v[i & 1] + dim * 128;
+    *reinterpret_cast<bf16x8*>(vr + 16 * ((2 * vc) ^ ((dim >> 1) & 7))) = to_bf16x8(vx[0], vx[1]);
+    *reinterpret_cast<bf16x8*>(vr + 16 * ((2 * vc + 1) ^ ((dim >> 1) & 7))) = to_bf16x8(vx[2], vx[3]);
+  };
+  const int kreg = (r & 3) + 4 * (r >> 3), krow = 16 * (kreg >> 3) + 8 * ((r >> 2) & 1) + (kreg & 7);
+  const int ko = krow * 256 + 16 * (hi ^ (krow & 15)), vo = r * 128 + 16 * (hi ^ ((r >> 1) & 7));
+  f32x16 sc[2];
+  bf16x8 pf[2][2] = {};
+  auto scores = [&](int i, int kt) {
+    f32x16 x = {};
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(sm.p.k[i & 1] + 8192 * kt + (ko ^ (32 * s))), qf[s], x, 0, 0, 0);
+    sc[kt] = x;
+  };
+  auto values = [&](int i, const bf16x8(&p)[2][2]) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(sm.p.v[i & 1] + 4096 * d + (vo ^ (64 * kt + 32 * s))),
+                                                        p[kt][s], o[d], 0, 0, 0);
+  };
+  float sub, sum[4];
+  auto weights = [&](int i, int kt, bf16x8(&p)[2]) {
+    const float* const vs = sm.p.s[i & 3][1] + 32 * kt + 8 * hi;
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const f32x4 f = *reinterpret_cast<const f32x4*>(vs + 16 * (e >> 3) + (e & 7));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = __builtin_amdgcn_exp2f(sc[kt][e + j] - sub);
+        sum[j] += x;
+        p[e >> 3][(e & 7) + j] = (__bf16)(x * f[j]);
+      }
+    }
+  };
+  if (np > 0) {
+    ask_k(0);
+    keep_k(0);
+    ask_k(1);
+    keep_k(1);
+    ask_k(2);
+    ask_v(0);
+    for (int i = tid; i < D * 8; i += 512) *reinterpret_cast<u32x4*>(sm.p.v[1] + 16 * i) = u32x4{0, 0, 0, 0};  // (page -1's weights are zeros)
+    lds_bar();
+    scores(0, 0);
+    scores(0, 1);
+    for (int i = 0; i < np; ++i) {
+      lds_bar();  // K(i + 1) and V(i - 1) are there, every wave is done with K(i) and V(i - 2)
+      keep_k(i + 2);
+      keep_v(i);
+      ask_k(i + 3);
+      ask_v(i + 1);
+      const int k0 = 64 * (p0 + i);
+      const float* const ks = sm.p.s[i & 3][0] + 8 * hi;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const f32x4 f = *reinterpret_cast<const f32x4*>(ks + 32 * kt + 16 * (e >> 3) + (e & 7));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[kt][e + j] *= f[j];
+        }
+      if (k0 + 64 > lo) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (k0 + 32 * kt + 16 * (e >> 3) + 8 * hi + (e & 7) >= limit) sc[kt][e] = -INFINITY;
+      }
+      float c0 = -INFINITY, c1 = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        c0 = fmaxf(c0, sc[0][e]);
+        c1 = fmaxf(c1, sc[1][e]);
+      }
+      float top = fmaxf(c0, c1);
+      const auto pr = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+      top = fmaxf(__uint_as_float(pr[0]), __uint_as_float(pr[1]));
+      // the maximum moves only when it would grow by more than 8: weights up to 2^8, and O is seldom rescaled
+      const bool up = top > m + 8.f;
+      const float mn = up ? top : m, alpha = up ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
+      sub = mn == -INFINITY ? 0.f : mn;
+      m = mn;
+      sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
+      bf16x8 pn[2][2];
+      values(i - 1, pf);
+      weights(i, 0, pn[0]);
+      scores(i + 1, 0);
+      weights(i, 1, pn[1]);
+      scores(i + 1, 1);
+      l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+      if (__ballot(up)) {
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
+      }
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) pf[kt][s] = pn[kt][s];
+    }
+    lds_bar();
+    values(np - 1, pf);
+  }
+  const int slot = a.tile_slot[tile];
+  l += __shfl_xor(l, 32, 64);
+  if (slot >= 0) {
+    if (!valid) return;
+    const size_t at = ((size_t)slot * a.nkv + kvh) * a.slot_rows + grow;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *reinterpret_cast<f32x4*>(a.part_o + at * D + 32 * d + 2 * e + 4 * hi) = f32x4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+    if (hi == 0) {
+      a.part_ml[2 * at] = m;
+      a.part_ml[2 * at + 1] = l;
+    }
+    return;
+  }
+  // rows leave through LDS, so that 16 lanes store one whole
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  lds_bar();
+  uint8_t* const ow = sm.o + w * (32 * kPitch);
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4)
+      *reinterpret_cast<u16x4*>(ow + r * kPitch + 2 * (32 * d + 2 * e + 4 * hi)) =
+          u16x4{f2bf(o[d][e] * inv), f2bf(o[d][e + 1] * inv), f2bf(o[d][e + 2] * inv), f2bf(o[d][e + 3] * inv)};
+  wave_lds_fence();
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int rr = 4 * j + (lane >> 4), gr = 32 * w + rr, c = lane & 15;
+    if (gr >= rows) continue;
+    uint16_t* const dst = a.out + (long)(tok0 + gr / a.G) * a.ldo + (kvh * a.G + gr % a.G) * D + 8 * c;
+    const u16x8 v = *reinterpret_cast<const u16x8*>(ow + rr * kPitch + 16 * c);
+    if (((uintptr_t)dst & 15) == 0) {
+      *reinterpret_cast<u16x8*>(dst) = v;
     } else {
-      const size_t at = ((size_t)slot * a.nkv + kvh) * a.slot_rows + rr;
-      put_part(st, i, m[i], l[i], a.part_o + at * D, a.part_ml + at * 2, r);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dst[e] = v[e];
     }
   }
 }
@@ -309,19 +514,19 @@ K8S_API int k8s_int8_attn_chunk(const void* q, long ldq, const void* k, const vo
                                 const int* m_np, int n_merge, float* part_o, float* part_ml, int slot_rows, void* stream) {
   using namespace k8s::q8;
   if (n_tiles <= 0) return 0;
-  if (nkv <= 0 || nq % nkv || BS <= 0 || (BS & 63) || NB <= 0 || rows <= 0 || rows > slot_rows) return (int)hipErrorInvalidValue;
+  if (nkv <= 0 || nq % nkv || BS <= 0 || (BS & 63) || NB <= 0 || rows <= 0 || rows > kRows || rows > slot_rows) return (int)hipErrorInvalidValue;
   if (n_merge > 0 && (!part_o || !part_ml)) return (int)hipErrorInvalidValue;
   AttnArgs a{};
   a.q = (const uint16_t*)q, a.ldq = ldq, a.k = (const uint8_t*)k, a.v = (const uint8_t*)v, a.ks = ks, a.vs = vs, a.bt = bt;
   a.bt_stride = bt_stride, a.NB = NB, a.ctx = ctx, a.q_start = q_start, a.nq = nq, a.nkv = nkv, a.G = nq / nkv, a.BS = BS;
   a.scale_log2 = scale * kLog2e, a.out = (uint16_t*)out, a.ldo = ldo, a.part_o = part_o, a.part_ml = part_ml;
   a.tile_seq = tile_seq, a.tile_tok0 = tile_tok0, a.tile_len = tile_len, a.tile_kv0 = tile_kv0, a.tile_kv1 = tile_kv1, a.tile_slot = tile_slot;
-  a.n_tiles = n_tiles, a.tile_waves = (rows + 15) / 16, a.m_tok0 = m_tok0, a.m_len = m_len, a.m_slot0 = m_slot0, a.m_np = m_np;
+  a.n_tiles = n_tiles, a.m_tok0 = m_tok0, a.m_len = m_len, a.m_slot0 = m_slot0, a.m_np = m_np;
   a.n_merge = n_merge, a.slot_rows = slot_rows;
   hipStream_t st = (hipStream_t)stream;
-  const long blocks = (long)n_tiles * nkv * a.tile_waves;
+  const long blocks = (long)n_tiles * nkv;
   if (blocks > 0x7fffffffL) return (int)hipErrorInvalidValue;
-  hipLaunchKernelGGL(chunk_kernel, dim3((unsigned)blocks), dim3(64), 0, st, a);
+  hipLaunchKernelGGL(chunk_kernel, dim3((unsigned)blocks), dim3(512), 0, st, a);
   if (n_merge > 0) hipLaunchKernelGGL(chunk_merge_kernel, dim3(n_merge * nkv, (rows + 1) / 2), dim3(2 * D), 0, st, a);
   return (int)hipGetLastError();
 }
