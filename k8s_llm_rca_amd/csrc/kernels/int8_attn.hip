@@ -238,14 +238,26 @@ __global__ void __launch_bounds__(D) reply_merge_kernel(AttnArgs a) {
 // 8 s .. 8 s + 7: the second operand of O^T += V^T P^T as they are.
 // LDS: a key's 256 bytes with 16-byte piece c at c ^ (key & 15), a dim's 128 bytes with piece c at c ^ ((dim >> 1) & 7): no bank
 // conflicts in either direction.
-// A turn has page i's softmax beside the products of its neighbours, so that the vector and the matrix units work at once: the
-// weights of its first 32 keys beside V(i - 1), those of the others beside the first half of K(i + 1), whose scores take the
-// registers that the weights have left.
+// A turn has page i's softmax beside the products of its neighbours, so that the vector and the matrix units work at once: scales,
+// maximum and the weights of the first 32 keys beside V(i - 1), the other weights beside the first half of K(i + 1), whose
+// scores take the registers that the weights have left, the staging beside its second half.  A fixed order of instructions holds it
+// together: left to the compiler, the products come first and the weights behind them (us of the four threads' chunks of
+// up to 2048 tokens over 4000: page after page 585, in turns 576, in this order 507).
 constexpr int kRows = 256, kPitch = 272;
+constexpr int AHEAD = 4;  // products that a fragment is read in front of its own
 struct ChunkLds {
   uint8_t k[2][64 * 256], v[2][D * 128];
   float s[4][2][64];  // keys' scales (with the softmax's, in powers of two), values'
 };
+template <int N>
+using ic = std::integral_constant<int, N>;
+template <int N, int J = 0, typename F>
+__device__ __forceinline__ void each(F&& f) {
+  if constexpr (J < N) {
+    f(ic<J>{});
+    each<N, J + 1>(f);
+  }
+}
 __device__ __forceinline__ void lds_bar() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
@@ -279,42 +291,42 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(AttnArgs a) {
     }
   }
   f32x16 o[4] = {};
-  float m = -INFINITY, l = 0.f;
+  float m = 0.f, l = 0.f;
 
   // staging: 16 dims of key tid >> 3, 16 keys of dim tid >> 2, a key's scales
   const int key = tid >> 3, kc = tid & 7, dim = tid >> 2, vc = tid & 3;
-  auto page_of = [&](int i, int& off) {
-    const int k0 = 64 * (p0 + min(i, np - 1));
-    off = k0 % a.BS;
-    return (size_t)min(max(__builtin_amdgcn_readfirstlane(bt[k0 / a.BS]), 0), a.NB - 1) * a.nkv + kvh;
-  };
+  const int step = a.nkv * a.BS;                            // keys of all heads in a block
+  const uint8_t* const kb = a.k + ((size_t)kvh * a.BS + key) * D + 16 * kc;
+  const uint8_t* const vb = a.v + ((size_t)kvh * D + dim) * a.BS + 16 * vc;
+  const float *const ksb = a.ks + kvh * a.BS + lane, *const vsb = a.vs + kvh * a.BS + lane;
+  // block ids of 64 pages, a lane each, and where the page that is asked for next lies (the last one for those behind the end)
+  auto ids_from = [&](int i) { return min(max(bt[64 * (p0 + min(i + lane, np - 1)) / a.BS], 0), a.NB - 1); };
+  int ids = 0, at_k = -1, off_k = 0, blk_k[3], offs[3];
   u32x4 kx, vx;
   float ksx = 0.f, vsx = 0.f;
   auto ask_k = [&](int i) {
-    int off;
-    const size_t page = page_of(i, off);
-    kx = *reinterpret_cast<const u32x4*>(a.k + (page * a.BS + off + key) * D + 16 * kc);
-    if (tid < 64) {
-      ksx = a.ks[page * a.BS + off + tid];
-      vsx = a.vs[page * a.BS + off + tid];
+    if (i < np) {
+      off_k += 64;
+      if (off_k >= a.BS) off_k = 0;
+      at_k = i;
     }
+    blk_k[0] = blk_k[1], blk_k[1] = blk_k[2], offs[0] = offs[1], offs[1] = offs[2];
+    blk_k[2] = __builtin_amdgcn_readlane(ids, at_k & 63), offs[2] = off_k;
+    const size_t first = (size_t)blk_k[2] * step + off_k;
+    kx = *reinterpret_cast<const u32x4*>(kb + first * D);
+    ksx = ksb[first];
+    vsx = vsb[first];
   };
-  auto ask_v = [&](int i) {
-    int off;
-    const size_t page = page_of(i, off);
-    vx = *reinterpret_cast<const u32x4*>(a.v + (page * D + dim) * a.BS + off + 16 * vc);
-  };
+  auto ask_v = [&] { vx = *reinterpret_cast<const u32x4*>(vb + (size_t)blk_k[0] * step * D + offs[0]); };  // of the page two behind
   auto keep_k = [&](int i) {
     uint8_t* const kr = sm.p.k[i & 1] + key * 256;
     *reinterpret_cast<bf16x8*>(kr + 16 * ((2 * kc) ^ (key & 15))) = to_bf16x8(kx[0], kx[1]);
     *reinterpret_cast<bf16x8*>(kr + 16 * ((2 * kc + 1) ^ (key & 15))) = to_bf16x8(kx[2], kx[3]);
-    if (tid < 64) {
-      // a key behind the context is nothing, whatever its scales say; a value that is no number makes its key's score none, so
-      // that the weights' factor is always a number (and a hidden key's product zero)
-      const bool in = 64 * (p0 + i) + tid < end, nan = vsx != vsx;
-      sm.p.s[i & 3][0][tid] = in ? (nan ? vsx : ksx * a.scale_log2) : 0.f;
-      sm.p.s[i & 3][1][tid] = in && !nan ? vsx : 0.f;
-    }
+    // a key behind the context is nothing, whatever its scales say; a value that is no number makes its key's score none, so
+    // that the weights' factor is always a number (and a hidden key's product zero).  All waves write the same.
+    const bool in = 64 * (p0 + i) + lane < end, nan = vsx != vsx;
+    sm.p.s[i & 3][0][lane] = in ? (nan ? vsx : ksx * a.scale_log2) : 0.f;
+    sm.p.s[i & 3][1][lane] = in && !nan ? vsx : 0.f;
   };
   auto keep_v = [&](int i) {
     uint8_t* const vr = sm.p.v[i & 1] + dim * 128;
@@ -325,106 +337,156 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(AttnArgs a) {
   const int ko = krow * 256 + 16 * (hi ^ (krow & 15)), vo = r * 128 + 16 * (hi ^ ((r >> 1) & 7));
   f32x16 sc[2];
   bf16x8 pf[2][2] = {};
-  auto scores = [&](int i, int kt) {
-    f32x16 x = {};
-#pragma unroll
-    for (int s = 0; s < 8; ++s)
-      x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(sm.p.k[i & 1] + 8192 * kt + (ko ^ (32 * s))), qf[s], x, 0, 0, 0);
-    sc[kt] = x;
+  // Product j of a turn: 0-15 V(i - 1) by the weights of its page, 16-31 K(i + 1) by Q.  Fragments are read AHEAD products ahead.
+  auto fragment = [&](auto J, int i) {
+    constexpr int j = decltype(J)::value;
+    if constexpr (j < 16)
+      return *reinterpret_cast<const bf16x8*>(sm.p.v[(i - 1) & 1] + 4096 * (j & 3) + (vo ^ (32 * (j >> 2))));
+    else
+      return *reinterpret_cast<const bf16x8*>(sm.p.k[(i + 1) & 1] + 8192 * ((j - 16) >> 3) + (ko ^ (32 * (j & 7))));
   };
-  auto values = [&](int i, const bf16x8(&p)[2][2]) {
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int d = 0; d < 4; ++d)
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(sm.p.v[i & 1] + 4096 * d + (vo ^ (64 * kt + 32 * s))),
-                                                        p[kt][s], o[d], 0, 0, 0);
-  };
-  float sub, sum[4];
-  auto weights = [&](int i, int kt, bf16x8(&p)[2]) {
-    const float* const vs = sm.p.s[i & 3][1] + 32 * kt + 8 * hi;
-#pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-      const f32x4 f = *reinterpret_cast<const f32x4*>(vs + 16 * (e >> 3) + (e & 7));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float x = __builtin_amdgcn_exp2f(sc[kt][e + j] - sub);
-        sum[j] += x;
-        p[e >> 3][(e & 7) + j] = (__bf16)(x * f[j]);
-      }
+  auto product = [&](auto J, const bf16x8& f) {
+    constexpr int j = decltype(J)::value;
+    if constexpr (j < 16) {
+      o[j & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, pf[j >> 3][(j >> 2) & 1], o[j & 3], 0, 0, 0);
+    } else {
+      if constexpr ((j & 7) == 0) sc[(j - 16) >> 3] = f32x16{};
+      sc[(j - 16) >> 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, qf[j & 7], sc[(j - 16) >> 3], 0, 0, 0);
     }
   };
   if (np > 0) {
+    ids = ids_from(0);
+    off_k = 64 * p0 % a.BS - 64;
     ask_k(0);
     keep_k(0);
     ask_k(1);
     keep_k(1);
     ask_k(2);
-    ask_v(0);
+    ask_v();
     for (int i = tid; i < D * 8; i += 512) *reinterpret_cast<u32x4*>(sm.p.v[1] + 16 * i) = u32x4{0, 0, 0, 0};  // (page -1's weights are zeros)
     lds_bar();
-    scores(0, 0);
-    scores(0, 1);
-    for (int i = 0; i < np; ++i) {
-      lds_bar();  // K(i + 1) and V(i - 1) are there, every wave is done with K(i) and V(i - 2)
-      keep_k(i + 2);
-      keep_v(i);
-      ask_k(i + 3);
-      ask_v(i + 1);
-      const int k0 = 64 * (p0 + i);
-      const float* const ks = sm.p.s[i & 3][0] + 8 * hi;
+    each<16>([&](auto J) { product(ic<decltype(J)::value + 16>{}, fragment(ic<decltype(J)::value + 16>{}, -1)); });
+    auto four = [](const float* f, int g) { return *reinterpret_cast<const f32x4*>(f + 16 * (g >> 1) + 4 * (g & 1)); };  // of a lane's scores 4g ..
+    auto hide = [&](int i) {  // keys that the row does not see
+      const int k0 = 64 * (p0 + i) + 8 * hi;
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const f32x4 f = *reinterpret_cast<const f32x4*>(ks + 32 * kt + 16 * (e >> 3) + (e & 7));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) sc[kt][e + j] *= f[j];
-        }
-      if (k0 + 64 > lo) {
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (k0 + 32 * kt + 16 * (e >> 3) + 8 * hi + (e & 7) >= limit) sc[kt][e] = -INFINITY;
-      }
+      for (int e = 0; e < 32; ++e)
+        if (k0 + 16 * (e >> 3) + (e & 7) >= limit) sc[e >> 4][e & 15] = -INFINITY;
+    };
+    auto largest = [&] {
       float c0 = -INFINITY, c1 = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         c0 = fmaxf(c0, sc[0][e]);
         c1 = fmaxf(c1, sc[1][e]);
       }
-      float top = fmaxf(c0, c1);
+      return fmaxf(c0, c1);
+    };
+    auto of_row = [](float top) {  // the two halves of a row
       const auto pr = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-      top = fmaxf(__uint_as_float(pr[0]), __uint_as_float(pr[1]));
-      // the maximum moves only when it would grow by more than 8: weights up to 2^8, and O is seldom rescaled
-      const bool up = top > m + 8.f;
-      const float mn = up ? top : m, alpha = up ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
-      sub = mn == -INFINITY ? 0.f : mn;
-      m = mn;
-      sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
-      bf16x8 pn[2][2];
-      values(i - 1, pf);
-      weights(i, 0, pn[0]);
-      scores(i + 1, 0);
-      weights(i, 1, pn[1]);
-      scores(i + 1, 1);
-      l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-      if (__ballot(up)) {
+      return fmaxf(__uint_as_float(pr[0]), __uint_as_float(pr[1]));
+    };
+    {
+      // where the row's weights begin: the largest score of the first page (a row without a key there has none at all)
+      const f32x16 raw[2] = {sc[0], sc[1]};
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        const f32x4 f = four(sm.p.s[0][0] + 8 * hi, g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[g >> 2][4 * (g & 3) + e] *= f[e];
+      }
+      hide(0);
+      const float top = of_row(largest());
+      m = top == -INFINITY ? 0.f : top;
+      sc[0] = raw[0], sc[1] = raw[1];
+    }
+    for (int i = 0; i < np; ++i) {
+      lds_bar();  // K(i + 1) and V(i - 1) are there, every wave is done with K(i) and V(i - 2)
+      const float *const ks = sm.p.s[i & 3][0] + 8 * hi, *const vs = sm.p.s[i & 3][1] + 8 * hi;
+      bf16x8 fr[AHEAD + 1];
+      uint32_t pn[16];
+      f32x4 fs[4];
+      // scales of four keys: of keys 4q .. of a lane, wanted by step q (q < 8), of values 4(q - 8) .., wanted by step 2 q - 8;
+      // read three steps in front
+      auto scale = [&](auto Q) {
+        constexpr int q = decltype(Q)::value;
+        fs[q & 3] = four(q < 8 ? ks : vs, q & 7);
+      };
+      float c[2] = {-INFINITY, -INFINITY}, sum[4] = {0.f, 0.f, 0.f, 0.f}, up = 0.f;
+      each<3>(scale);
+      each<AHEAD>([&](auto J) { fr[J] = fragment(J, i); });
+      each<32>([&](auto Jc) {
+        constexpr int j = decltype(Jc)::value;
+        if constexpr (j + AHEAD < 32) fr[(j + AHEAD) % (AHEAD + 1)] = fragment(ic<j + AHEAD>{}, i);
+        if constexpr (j < 5)
+          scale(ic<j + 3>{});
+        else if constexpr (j < 20 && (j & 1))
+          scale(ic<(j + 11) / 2>{});
+        product(Jc, fr[j % (AHEAD + 1)]);
+        if constexpr (j < 8) {  // four scores of the lane, above what the row's weights stand on
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x = fmaf(sc[j >> 2][4 * (j & 3) + e], fs[j & 3][e], -m);
+            asm volatile("" : "+v"(x));  // (not made again from the sum and the scale, which would stay in registers for it)
+            sc[j >> 2][4 * (j & 3) + e] = x;
+            c[e & 1] = fmaxf(c[e & 1], x);
+          }
+        } else if constexpr (j < 24) {  // two weights
+          if constexpr (j == 8) {
+            float top = fmaxf(c[0], c[1]);
+            if (64 * (p0 + i) + 64 > lo) {
+              hide(i);
+              top = largest();
+            }
+            top = of_row(top);
+            // where a row grows by more than 8, its weights stand on its new maximum from here on: weights up to 2^8
+            if (__ballot(top > 8.f)) {
+              up = top > 8.f ? top : 0.f;
+              m += up;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) sc[e >> 4][e & 15] -= up;
+            }
+          }
+          constexpr int t = j - 8, kt = t >> 3, e = 2 * (t & 7);
+          const float x0 = __builtin_amdgcn_exp2f(sc[kt][e]), x1 = __builtin_amdgcn_exp2f(sc[kt][e + 1]);
+          sum[2 * (t & 1)] += x0;
+          sum[2 * (t & 1) + 1] += x1;
+          typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+          uint32_t two = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)(x0 * fs[(t >> 1) & 3][e & 3]), (__bf16)(x1 * fs[(t >> 1) & 3][(e & 3) + 1])});
+          // (wanted in the next turn only: computed here all the same, beside the products)
+          asm volatile("" : "+v"(two), "+v"(sum[2 * (t & 1)]), "+v"(sum[2 * (t & 1) + 1]));
+          pn[t] = two;
+        } else if constexpr (j == 24) {
+          keep_k(i + 2);
+        } else if constexpr (j == 27) {
+          ask_k(i + 3);
+        } else if constexpr (j == 28) {
+          keep_v(i);
+        } else if constexpr (j == 30) {
+          ask_v();
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      if (((i + 4) & 63) == 0 && i + 4 < np) ids = ids_from(i + 4);
+      if (__ballot(up != 0.f)) {
+        const float alpha = __builtin_amdgcn_exp2f(-up);
+        l *= alpha;
 #pragma unroll
         for (int d = 0; d < 4; ++d)
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
       }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int s = 0; s < 2; ++s) pf[kt][s] = pn[kt][s];
+        for (int s = 0; s < 2; ++s) {
+          const uint32_t* const t = pn + 8 * kt + 4 * s;
+          pf[kt][s] = __builtin_bit_cast(bf16x8, u32x4{t[0], t[1], t[2], t[3]});
+        }
     }
     lds_bar();
-    values(np - 1, pf);
+    each<16>([&](auto J) { product(J, fragment(J, np)); });
   }
   const int slot = a.tile_slot[tile];
   l += __shfl_xor(l, 32, 64);
@@ -437,7 +499,7 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(AttnArgs a) {
       for (int e = 0; e < 16; e += 4)
         *reinterpret_cast<f32x4*>(a.part_o + at * D + 32 * d + 2 * e + 4 * hi) = f32x4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
     if (hi == 0) {
-      a.part_ml[2 * at] = m;
+      a.part_ml[2 * at] = l == 0.f ? -INFINITY : m;  // (a row without a key in this run)
       a.part_ml[2 * at + 1] = l;
     }
     return;
