@@ -64,47 +64,78 @@ __device__ __forceinline__ void load_q(State& st, const AttnArgs& a, long row, i
 }
 
 // Keys [k0, k1) (k0 a multiple of 64) of one sequence; row lane & 15 sees keys below lim, every row those below kmin.
+// A chunk's keys and values make room for the next chunk's as soon as they are used, so that a wave always has 8 to 16 KB on the way.
+template <bool NT>
+__device__ __forceinline__ u32x4 get(const uint8_t* p) {
+  if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+  return *reinterpret_cast<const u32x4*>(p);
+}
+#ifndef RNT
+#define RNT 1
+#endif
 __device__ __forceinline__ void walk(State& st, const AttnArgs& a, const int* bt, int kvh, int k0, int k1, int kmin, int lim, int lane) {
-  const int r = lane & 15, g = lane >> 4;
-  for (int kb = k0; kb < k1; kb += 64) {
-    const int blk = min(max(__builtin_amdgcn_readfirstlane(bt[kb / a.BS]), 0), a.NB - 1);
-    const size_t page = (size_t)blk * a.nkv + kvh;
-    const int off = kb % a.BS;
-    const uint8_t* kp = a.k + (page * a.BS + off) * D + 16 * g;
-    const uint8_t* vp = a.v + page * D * a.BS + off + 16 * g;
-    const float* ksp = a.ks + page * a.BS + off + 16 * g;
-    const float* vsp = a.vs + page * a.BS + off + 16 * g;
-    u32x4 kf[4][2], vf[8];
-    f32x4 ks[4], vs[4];
+  const int r = lane & 15, g = lane >> 4, n = (k1 - k0 + 63) >> 6;
+  if (n <= 0) return;
+  const uint8_t* const kb = a.k + ((size_t)kvh * a.BS + 16 * (r >> 2) + (r & 3)) * D + 16 * g;
+  const uint8_t* const vb = a.v + ((size_t)kvh * D + r) * a.BS + 16 * g;
+  const float *const ksb = a.ks + kvh * a.BS + 16 * g, *const vsb = a.vs + kvh * a.BS + 16 * g;
+  // block ids of 64 chunks, a lane each
+  auto ids_from = [&](int c) { return min(max(bt[(k0 + 64 * min(c + lane, n - 1)) / a.BS], 0), a.NB - 1); };
+  int ids = ids_from(0), off = k0 % a.BS;
+  u32x4 kf[4][2], vf[8];
+  f32x4 ks[4], vs[4];
+  auto ask_k = [&](size_t at) {
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const int key = 16 * (r >> 2) + 4 * t + (r & 3);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) kf[t][c] = *reinterpret_cast<const u32x4*>(kp + key * D + 64 * c);
-      ks[t] = *reinterpret_cast<const f32x4*>(ksp + 4 * t);
-      vs[t] = *reinterpret_cast<const f32x4*>(vsp + 4 * t);
+      for (int c = 0; c < 2; ++c) kf[t][c] = get<RNT>(kb + (at + 4 * t) * D + 64 * c);
+      ks[t] = *reinterpret_cast<const f32x4*>(ksb + at + 4 * t);
     }
+  };
+  auto ask_v = [&](size_t at, int off) {
+    const uint8_t* const p = vb + (at - off) * D + off;
 #pragma unroll
-    for (int d = 0; d < 8; ++d) vf[d] = *reinterpret_cast<const u32x4*>(vp + (16 * d + r) * a.BS);
+    for (int d = 0; d < 8; ++d) vf[d] = get<RNT>(p + 16 * d * a.BS);
+  };
+  auto ask_vs = [&](size_t at) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) vs[t] = *reinterpret_cast<const f32x4*>(vsb + at + 4 * t);
+  };
+  const size_t step = (size_t)a.nkv * a.BS;  // keys of all heads in a block
+  {
+    const size_t at = __builtin_amdgcn_readlane(ids, 0) * step + off;
+    ask_k(at);
+    ask_vs(at);
+    ask_v(at, off);
+  }
+  for (int c = 0; c < n; ++c) {
+    const int kb0 = k0 + 64 * c;
+    if (c + 1 < n) {
+      off += 64;
+      if (off >= a.BS) off = 0;
+      if (((c + 1) & 63) == 0) ids = ids_from(c + 1);
+    }
+    const size_t at = __builtin_amdgcn_readlane(ids, min(c + 1, n - 1) & 63) * step + off;  // (the last chunk asks for itself again)
     f32x4 sc[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16x8(kf[t][c][0], kf[t][c][1]), st.qf[2 * c], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16x8(kf[t][c][2], kf[t][c][3]), st.qf[2 * c + 1], acc, 0, 0, 0);
+      for (int e = 0; e < 2; ++e) {
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16x8(kf[t][e][0], kf[t][e][1]), st.qf[2 * e], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16x8(kf[t][e][2], kf[t][e][3]), st.qf[2 * e + 1], acc, 0, 0, 0);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) sc[t][i] = acc[i] * (ks[t][i] * a.scale_log2);
     }
-    if (kb + 64 > kmin) {  // keys that a row does not see: no weight, whatever stands there (a scale may be a NaN)
+    __builtin_amdgcn_sched_barrier(0);
+    ask_k(at);
+    if (kb0 + 64 > kmin) {  // keys that a row does not see: no weight, whatever stands there (a scale may be a NaN)
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (kb + 16 * g + 4 * t + i >= lim) sc[t][i] = -INFINITY, vs[t][i] = 0.f;
-        }
+        for (int i = 0; i < 4; ++i)
+          if (kb0 + 16 * g + 4 * t + i >= lim) sc[t][i] = -INFINITY, vs[t][i] = 0.f;
     }
     float top = -INFINITY;
 #pragma unroll
@@ -139,11 +170,14 @@ __device__ __forceinline__ void walk(State& st, const AttnArgs& a, const int* bt
 #pragma unroll
         for (int i = 0; i < 4; ++i) st.o[d][i] *= ar[i];
     }
+    ask_vs(at);
 #pragma unroll
     for (int d = 0; d < 8; ++d) {
       st.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[0], to_bf16x8(vf[d][0], vf[d][1]), st.o[d], 0, 0, 0);
       st.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[1], to_bf16x8(vf[d][2], vf[d][3]), st.o[d], 0, 0, 0);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    ask_v(at, off);
   }
 }
 
@@ -213,30 +247,59 @@ __global__ void __launch_bounds__(64, 2) reply_kernel(AttnArgs a) {
       for (int c = lane; c < a.nq * D; c += 64) a.out[a.q_start[s] * a.ldo + c] = 0;
 }
 
-// rows of more than one part: grid (nq, S), a thread a dim
-__global__ void __launch_bounds__(D) reply_merge_kernel(AttnArgs a) {
-  const int head = blockIdx.x, seq = blockIdx.y, d = threadIdx.x;
+// The parts of a row: 32 lanes have four dims each, the groups of 32 every G-th part; they meet in LDS.  Parts are added in an
+// order that only their count decides.
+template <int G>
+__device__ __forceinline__ void join_parts(const float* po, const float* pml, size_t at, size_t step, int np, uint16_t* out) {
+  __shared__ f32x4 so[G][32];
+  __shared__ float sl[G];
+  const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
+  float M = -INFINITY, L = 0.f;
+  f32x4 O = {0.f, 0.f, 0.f, 0.f};
+  {
+    for (int p = c; p < np; p += 32) M = fmaxf(M, pml[(at + p * step) * 2]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+#pragma unroll 4
+    for (int p = g; p < np; p += G) {
+      const float m = pml[(at + p * step) * 2], l = pml[(at + p * step) * 2 + 1];
+      const f32x4 v = *reinterpret_cast<const f32x4*>(po + (at + p * step) * D + 4 * c);
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+      L = fmaf(l, f, L);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) O[e] = fmaf(v[e], f, O[e]);
+    }
+  }
+  so[g][c] = O;
+  if (c == 0) sl[g] = L;
+  __syncthreads();
+  if (g) return;
+#pragma unroll
+  for (int k = 1; k < G; ++k) {
+    L += sl[k];
+    O += so[k][c];
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[4 * c + e] = f2bf(O[e] * inv);
+}
+
+// rows of more than one part: grid (nq, S)
+__global__ void __launch_bounds__(256) reply_merge_kernel(AttnArgs a) {
+  const int head = blockIdx.x, seq = blockIdx.y;
   const int part_size = a.d_items ? a.d_items[1] : a.part_size;
   const int np = min(a.n_parts, (a.ctx[seq] + part_size - 1) / part_size);
   if (np <= 1) return;
-  const size_t at = ((size_t)seq * a.nq + head) * a.n_parts;
-  float M = -INFINITY, L = 0.f, O = 0.f;
-  for (int p = 0; p < np; ++p) M = fmaxf(M, a.part_ml[(at + p) * 2]);
-  for (int p = 0; p < np; ++p) {
-    const float m = a.part_ml[(at + p) * 2], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
-    L = fmaf(a.part_ml[(at + p) * 2 + 1], f, L);
-    O = fmaf(a.part_o[(at + p) * D + d], f, O);
-  }
-  a.out[a.q_start[seq] * a.ldo + head * D + d] = f2bf(L == 0.f ? 0.f : O / L);
+  join_parts<8>(a.part_o, a.part_ml, ((size_t)seq * a.nq + head) * a.n_parts, 1, np, a.out + a.q_start[seq] * a.ldo + head * D);
 }
 
 // ------------------------------------------------------------------ chunks
 // A workgroup holds up to 256 rows (token, q head) of one kv head, 32 a wave, and walks pages of 64 keys.  Keys and values are made
-// bf16 once for all waves on their way into LDS (two pages each): 16 of each a thread, asked for a page ahead.
+// bf16 once for all waves on their way into LDS: 16 of each a thread, asked for a page ahead.
 // v_mfma_f32_32x32x16_bf16, S^T = K Q^T: row rho of the 32-key half kt is key 32 kt + 16 (reg >> 3) + 8 hi + (reg & 7) with
 // reg = (rho & 3) + 4 (rho >> 3), hi = (rho >> 2) & 1, so that a lane has one row's keys 16 s + 8 hi .. + 7 in registers
 // 8 s .. 8 s + 7: the second operand of O^T += V^T P^T as they are.
-// LDS: a key's 256 bytes with 16-byte piece c at c ^ (key & 15), a dim's 128 bytes with piece c at c ^ ((dim >> 1) & 7): no bank
+// LDS (three pages of each, so that a turn's first fragments are read in front of its barrier): a key's 256 bytes with 16-byte piece c at c ^ (key & 15), a dim's 128 bytes with piece c at c ^ ((dim >> 1) & 7): no bank
 // conflicts in either direction.
 // A turn has page i's softmax beside the products of its neighbours, so that the vector and the matrix units work at once: scales,
 // maximum and the weights of the first 32 keys beside V(i - 1), the other weights beside the first half of K(i + 1), whose
@@ -244,9 +307,9 @@ __global__ void __launch_bounds__(D) reply_merge_kernel(AttnArgs a) {
 // together: left to the compiler, the products come first and the weights behind them (us of the four threads' chunks of
 // up to 2048 tokens over 4000: page after page 585, in turns 576, in this order 507).
 constexpr int kRows = 256, kPitch = 272;
-constexpr int AHEAD = 4;  // products that a fragment is read in front of its own
+constexpr int AHEAD = 3;  // products that a fragment is read in front of its own
 struct ChunkLds {
-  uint8_t k[2][64 * 256], v[2][D * 128];
+  uint8_t k[3][64 * 256], v[3][D * 128];
   float s[4][2][64];  // keys' scales (with the softmax's, in powers of two), values'
 };
 template <int N>
@@ -318,8 +381,8 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(AttnArgs a) {
     vsx = vsb[first];
   };
   auto ask_v = [&] { vx = *reinterpret_cast<const u32x4*>(vb + (size_t)blk_k[0] * step * D + offs[0]); };  // of the page two behind
-  auto keep_k = [&](int i) {
-    uint8_t* const kr = sm.p.k[i & 1] + key * 256;
+  auto keep_k = [&](int i, int slot) {
+    uint8_t* const kr = sm.p.k[slot] + key * 256;
     *reinterpret_cast<bf16x8*>(kr + 16 * ((2 * kc) ^ (key & 15))) = to_bf16x8(kx[0], kx[1]);
     *reinterpret_cast<bf16x8*>(kr + 16 * ((2 * kc + 1) ^ (key & 15))) = to_bf16x8(kx[2], kx[3]);
     // a key behind the context is nothing, whatever its scales say; a value that is no number makes its key's score none, so
@@ -328,8 +391,8 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(AttnArgs a) {
     sm.p.s[i & 3][0][lane] = in ? (nan ? vsx : ksx * a.scale_log2) : 0.f;
     sm.p.s[i & 3][1][lane] = in && !nan ? vsx : 0.f;
   };
-  auto keep_v = [&](int i) {
-    uint8_t* const vr = sm.p.v[i & 1] + dim * 128;
+  auto keep_v = [&](int slot) {
+    uint8_t* const vr = sm.p.v[slot] + dim * 128;
     *reinterpret_cast<bf16x8*>(vr + 16 * ((2 * vc) ^ ((dim >> 1) & 7))) = to_bf16x8(vx[0], vx[1]);
     *reinterpret_cast<bf16x8*>(vr + 16 * ((2 * vc + 1) ^ ((dim >> 1) & 7))) = to_bf16x8(vx[2], vx[3]);
   };
@@ -337,13 +400,14 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(AttnArgs a) {
   const int ko = krow * 256 + 16 * (hi ^ (krow & 15)), vo = r * 128 + 16 * (hi ^ ((r >> 1) & 7));
   f32x16 sc[2];
   bf16x8 pf[2][2] = {};
-  // Product j of a turn: 0-15 V(i - 1) by the weights of its page, 16-31 K(i + 1) by Q.  Fragments are read AHEAD products ahead.
-  auto fragment = [&](auto J, int i) {
+  // Product j of a turn: 0-15 V(i - 1), in its place `vp`, by the weights of its page, 16-31 K(i + 1), in `kp`, by Q.  Fragments are
+  // read AHEAD products ahead.
+  auto fragment = [&](auto J, int vp, int kp) {
     constexpr int j = decltype(J)::value;
     if constexpr (j < 16)
-      return *reinterpret_cast<const bf16x8*>(sm.p.v[(i - 1) & 1] + 4096 * (j & 3) + (vo ^ (32 * (j >> 2))));
+      return *reinterpret_cast<const bf16x8*>(sm.p.v[vp] + 4096 * (j & 3) + (vo ^ (32 * (j >> 2))));
     else
-      return *reinterpret_cast<const bf16x8*>(sm.p.k[(i + 1) & 1] + 8192 * ((j - 16) >> 3) + (ko ^ (32 * (j & 7))));
+      return *reinterpret_cast<const bf16x8*>(sm.p.k[kp] + 8192 * ((j - 16) >> 3) + (ko ^ (32 * (j & 7))));
   };
   auto product = [&](auto J, const bf16x8& f) {
     constexpr int j = decltype(J)::value;
@@ -358,14 +422,18 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(AttnArgs a) {
     ids = ids_from(0);
     off_k = 64 * p0 % a.BS - 64;
     ask_k(0);
-    keep_k(0);
+    keep_k(0, 0);
     ask_k(1);
-    keep_k(1);
+    keep_k(1, 1);
     ask_k(2);
     ask_v();
-    for (int i = tid; i < D * 8; i += 512) *reinterpret_cast<u32x4*>(sm.p.v[1] + 16 * i) = u32x4{0, 0, 0, 0};  // (page -1's weights are zeros)
+    keep_k(2, 2);
+    keep_v(0);
+    ask_k(3);
+    ask_v();
+    for (int i = tid; i < D * 8; i += 512) *reinterpret_cast<u32x4*>(sm.p.v[2] + 16 * i) = u32x4{0, 0, 0, 0};  // (page -1's weights are zeros)
     lds_bar();
-    each<16>([&](auto J) { product(ic<decltype(J)::value + 16>{}, fragment(ic<decltype(J)::value + 16>{}, -1)); });
+    each<16>([&](auto J) { product(ic<decltype(J)::value + 16>{}, fragment(ic<decltype(J)::value + 16>{}, 0, 0)); });
     auto four = [](const float* f, int g) { return *reinterpret_cast<const f32x4*>(f + 16 * (g >> 1) + 4 * (g & 1)); };  // of a lane's scores 4g ..
     auto hide = [&](int i) {  // keys that the row does not see
       const int k0 = 64 * (p0 + i) + 8 * hi;
@@ -400,29 +468,36 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(AttnArgs a) {
       m = top == -INFINITY ? 0.f : top;
       sc[0] = raw[0], sc[1] = raw[1];
     }
+    bf16x8 fr[4];
+    f32x4 fs[4];
+    // scales of four keys: of keys 4q .. of a lane, wanted by step q (q < 8), of values 4(q - 8) .., wanted by step 2 q - 8; read
+    // three steps in front
+    auto scale = [&](auto Q, int i) {
+      constexpr int q = decltype(Q)::value;
+      fs[q & 3] = four(sm.p.s[i & 3][q >> 3] + 8 * hi, q & 7);
+    };
+    each<3>([&](auto J) {
+      scale(J, 0);
+      fr[J] = fragment(J, 2, 1);
+    });
+    int s0 = 0, s1 = 1, s2 = 2;  // i, i + 1 and i + 2 by three
     for (int i = 0; i < np; ++i) {
-      lds_bar();  // K(i + 1) and V(i - 1) are there, every wave is done with K(i) and V(i - 2)
-      const float *const ks = sm.p.s[i & 3][0] + 8 * hi, *const vs = sm.p.s[i & 3][1] + 8 * hi;
-      bf16x8 fr[AHEAD + 1];
+      lds_bar();  // K(i + 2) and V(i) are there, every wave is done with K(i) and V(i - 2)
       uint32_t pn[16];
-      f32x4 fs[4];
-      // scales of four keys: of keys 4q .. of a lane, wanted by step q (q < 8), of values 4(q - 8) .., wanted by step 2 q - 8;
-      // read three steps in front
-      auto scale = [&](auto Q) {
-        constexpr int q = decltype(Q)::value;
-        fs[q & 3] = four(q < 8 ? ks : vs, q & 7);
-      };
       float c[2] = {-INFINITY, -INFINITY}, sum[4] = {0.f, 0.f, 0.f, 0.f}, up = 0.f;
-      each<3>(scale);
-      each<AHEAD>([&](auto J) { fr[J] = fragment(J, i); });
       each<32>([&](auto Jc) {
         constexpr int j = decltype(Jc)::value;
-        if constexpr (j + AHEAD < 32) fr[(j + AHEAD) % (AHEAD + 1)] = fragment(ic<j + AHEAD>{}, i);
+        if constexpr (j + AHEAD < 32)
+          fr[(j + AHEAD) & 3] = fragment(ic<j + AHEAD>{}, s2, s1);
+        else
+          fr[(j + AHEAD) & 3] = fragment(ic<j + AHEAD - 32>{}, s0, s2);  // the next turn's
         if constexpr (j < 5)
-          scale(ic<j + 3>{});
+          scale(ic<j + 3>{}, i);
         else if constexpr (j < 20 && (j & 1))
-          scale(ic<(j + 11) / 2>{});
-        product(Jc, fr[j % (AHEAD + 1)]);
+          scale(ic<(j + 11) / 2>{}, i);
+        else if constexpr (j >= 29)
+          scale(ic<j - 29>{}, i + 1);
+        product(Jc, fr[j & 3]);
         if constexpr (j < 8) {  // four scores of the lane, above what the row's weights stand on
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -457,17 +532,17 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(AttnArgs a) {
           asm volatile("" : "+v"(two), "+v"(sum[2 * (t & 1)]), "+v"(sum[2 * (t & 1) + 1]));
           pn[t] = two;
         } else if constexpr (j == 24) {
-          keep_k(i + 2);
+          keep_k(i + 3, s0);
         } else if constexpr (j == 27) {
-          ask_k(i + 3);
+          ask_k(i + 4);
         } else if constexpr (j == 28) {
-          keep_v(i);
+          keep_v(s1);
         } else if constexpr (j == 30) {
           ask_v();
         }
         __builtin_amdgcn_sched_barrier(0);
       });
-      if (((i + 4) & 63) == 0 && i + 4 < np) ids = ids_from(i + 4);
+      if (((i + 5) & 63) == 0 && i + 5 < np) ids = ids_from(i + 5);
       if (__ballot(up != 0.f)) {
         const float alpha = __builtin_amdgcn_exp2f(-up);
         l *= alpha;
@@ -484,9 +559,14 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(AttnArgs a) {
           const uint32_t* const t = pn + 8 * kt + 4 * s;
           pf[kt][s] = __builtin_bit_cast(bf16x8, u32x4{t[0], t[1], t[2], t[3]});
         }
+      const int s3 = s0;
+      s0 = s1, s1 = s2, s2 = s3;
     }
-    lds_bar();
-    each<16>([&](auto J) { product(J, fragment(J, np)); });
+    each<16>([&](auto J) {  // (V(np - 1) is at s2)
+      constexpr int j = decltype(J)::value;
+      product(J, fr[j & 3]);
+      if constexpr (j + AHEAD < 16) fr[(j + AHEAD) & 3] = fragment(ic<j + AHEAD>{}, s2, 0);
+    });
   }
   const int slot = a.tile_slot[tile];
   l += __shfl_xor(l, 32, 64);
@@ -530,20 +610,12 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(AttnArgs a) {
   }
 }
 
-// grid (n_merge * nkv, rows / 2): two rows a workgroup, a thread a dim
-__global__ void __launch_bounds__(2 * D) chunk_merge_kernel(AttnArgs a) {
-  const int kvh = blockIdx.x % a.nkv, mi = blockIdx.x / a.nkv, row = blockIdx.y * 2 + (threadIdx.x >> 7), d = threadIdx.x & (D - 1);
+// rows of split tiles: grid (n_merge * nkv, rows)
+__global__ void __launch_bounds__(64) chunk_merge_kernel(AttnArgs a) {
+  const int kvh = blockIdx.x % a.nkv, mi = blockIdx.x / a.nkv, row = blockIdx.y;
   if (row >= a.m_len[mi] * a.G) return;
-  const int slot0 = a.m_slot0[mi], np = a.m_np[mi];
-  float M = -INFINITY, L = 0.f, O = 0.f;
-  auto at = [&](int p) { return ((size_t)(slot0 + p) * a.nkv + kvh) * a.slot_rows + row; };
-  for (int p = 0; p < np; ++p) M = fmaxf(M, a.part_ml[at(p) * 2]);
-  for (int p = 0; p < np; ++p) {
-    const float m = a.part_ml[at(p) * 2], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
-    L = fmaf(a.part_ml[at(p) * 2 + 1], f, L);
-    O = fmaf(a.part_o[at(p) * D + d], f, O);
-  }
-  a.out[(long)(a.m_tok0[mi] + row / a.G) * a.ldo + (kvh * a.G + row % a.G) * D + d] = f2bf(L == 0.f ? 0.f : O / L);
+  join_parts<2>(a.part_o, a.part_ml, ((size_t)a.m_slot0[mi] * a.nkv + kvh) * a.slot_rows + row, (size_t)a.nkv * a.slot_rows, a.m_np[mi],
+                a.out + (long)(a.m_tok0[mi] + row / a.G) * a.ldo + (kvh * a.G + row % a.G) * D);
 }
 
 }  // namespace q8
@@ -564,7 +636,7 @@ K8S_API int k8s_int8_attn_reply(const void* q, long ldq, const void* k, const vo
   a.part_size = part_size, a.items = (const int4*)items, a.n_items = n_items, a.d_items = d_items;
   hipStream_t st = (hipStream_t)stream;
   hipLaunchKernelGGL(reply_kernel, dim3(grid), dim3(64), 0, st, a);
-  if (n_parts > 1) hipLaunchKernelGGL(reply_merge_kernel, dim3(nq, S), dim3(D), 0, st, a);
+  if (n_parts > 1) hipLaunchKernelGGL(reply_merge_kernel, dim3(nq, S), dim3(256), 0, st, a);
   return (int)hipGetLastError();
 }
 
@@ -589,6 +661,6 @@ K8S_API int k8s_int8_attn_chunk(const void* q, long ldq, const void* k, const vo
   const long blocks = (long)n_tiles * nkv;
   if (blocks > 0x7fffffffL) return (int)hipErrorInvalidValue;
   hipLaunchKernelGGL(chunk_kernel, dim3((unsigned)blocks), dim3(512), 0, st, a);
-  if (n_merge > 0) hipLaunchKernelGGL(chunk_merge_kernel, dim3(n_merge * nkv, (rows + 1) / 2), dim3(2 * D), 0, st, a);
+  if (n_merge > 0) hipLaunchKernelGGL(chunk_merge_kernel, dim3(n_merge * nkv, rows), dim3(64), 0, st, a);
   return (int)hipGetLastError();
 }

@@ -19,60 +19,160 @@ struct WriteArgs {
   long cap;  // slots of the pool
 };
 
-// Eight lanes a head: lane j has dims 8j .. 8j+7 and their partners 64 on.
-__global__ void __launch_bounds__(256) write_kernel(WriteArgs a) {
-  const int heads = a.nq + 2 * a.nkv, j = threadIdx.x & 7;
-  const long unit = (blockIdx.x * 256L + threadIdx.x) >> 3;
-  const bool live = unit < (long)a.T * heads;  // (all eight lanes of a head, so that the exchange below has its partners)
-  if (!live) return;
-  const int t = (int)(unit / heads), h = (int)(unit % heads);
-  uint16_t* const p = a.qkv + (size_t)t * a.ld + h * 128 + 8 * j;
-  const u16x8 lo = *reinterpret_cast<const u16x8*>(p), hi = *reinterpret_cast<const u16x8*>(p + 64);
-  float x[8], y[8];
-  if (h < a.nq + a.nkv) {
-    // (a position outside the table takes its last row: no read behind it)
-    const int ps = min(max(a.pos[t], 0), a.max_pos - 1);
-    const float* cs = a.cos_sin + (size_t)ps * 128 + 8 * j;
+constexpr int kTokens = 64, kCols = kTokens + 16, kPitch = 84;  // of a workgroup that writes values; bytes of its LDS rows
+
+// Whether the row is kept, and where.
+__device__ __forceinline__ int slot_of(const WriteArgs& a, int t) {
+  const int s = t < a.T && a.slots ? a.slots[t] : -1;
+  return s < a.cap ? s : -1;
+}
+
+// A wave a token, eight lanes a head (lane j has dims 8j .. 8j+7 and their partners 64 on), so that a lane reads its cosines
+// once for all heads.  VALUES: the value heads, too, byte by byte.
+template <bool VALUES>
+__device__ __forceinline__ void rotate(const WriteArgs& a, int t, int lane) {
+  if (t >= a.T) return;
+  const int j = lane & 7, heads = a.nq + (VALUES ? 2 : 1) * a.nkv;
+  uint16_t* const row = a.qkv + (size_t)t * a.ld + 8 * j;
+  // (a position outside the table takes its last row: no read behind it)
+  const float* const cs = a.cos_sin + (size_t)min(max(a.pos[t], 0), a.max_pos - 1) * 128 + 8 * j;
+  const int slot = slot_of(a, t), blk = max(slot, 0) / a.BS, off = max(slot, 0) - blk * a.BS;
+  f32x4 co[2], si[2];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) rope_pair(bf2f(lo[e]), bf2f(hi[e]), cs[e], cs[64 + e], x[e], y[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = bf2f(lo[e]), y[e] = bf2f(hi[e]);
+  for (int e = 0; e < 2; ++e) {
+    co[e] = *reinterpret_cast<const f32x4*>(cs + 4 * e);
+    si[e] = *reinterpret_cast<const f32x4*>(cs + 64 + 4 * e);
   }
-  if (h < a.nq) {
-    u16x8 o0, o1;
+  constexpr int U = 5;
+  for (int h0 = lane >> 3; h0 < heads; h0 += 8 * U) {
+    u16x8 lo[U], hi[U];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o0[e] = f2bf(x[e]), o1[e] = f2bf(y[e]);
-    *reinterpret_cast<u16x8*>(p) = o0;
-    *reinterpret_cast<u16x8*>(p + 64) = o1;
-    return;
+    for (int u = 0; u < U; ++u) {
+      const uint16_t* const p = row + min(h0 + 8 * u, heads - 1) * 128;
+      lo[u] = *reinterpret_cast<const u16x8*>(p);
+      hi[u] = *reinterpret_cast<const u16x8*>(p + 64);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + 8 * u;
+      if (h >= heads) break;
+      float x[8], y[8];
+      const bool turned = !VALUES || h < a.nq + a.nkv;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = bf2f(lo[u][e]), y[e] = bf2f(hi[u][e]);
+        if (turned) rope_pair(x[e], y[e], co[e >> 2][e & 3], si[e >> 2][e & 3], x[e], y[e]);
+      }
+      if (h < a.nq) {
+        u16x8 o0, o1;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o0[e] = f2bf(x[e]), o1[e] = f2bf(y[e]);
+        *reinterpret_cast<u16x8*>(row + h * 128) = o0;
+        *reinterpret_cast<u16x8*>(row + h * 128 + 64) = o1;
+        continue;
+      }
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, max(abs_bits(x[e]), abs_bits(y[e])));
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+      if (slot < 0) continue;
+      const Step s = row_step(top);
+      const u32x2 q0 = pack8(x, s), q1 = pack8(y, s);
+      const size_t page = (size_t)blk * a.nkv + h - a.nq - (turned ? 0 : a.nkv), at = page * a.BS + off;
+      if (turned) {
+        *reinterpret_cast<u32x2*>(a.k + at * 128 + 8 * j) = q0;
+        *reinterpret_cast<u32x2*>(a.k + at * 128 + 64 + 8 * j) = q1;
+      } else {
+        uint8_t* const d = a.v + (page * 128 + 8 * j) * a.BS + off;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          d[(size_t)e * a.BS] = (uint8_t)(q0[e >> 2] >> (8 * (e & 3)));
+          d[(size_t)(64 + e) * a.BS] = (uint8_t)(q1[e >> 2] >> (8 * (e & 3)));
+        }
+      }
+      if (j == 0) (turned ? a.ks : a.vs)[at] = s.scale;
+    }
   }
-  uint32_t top = 0;
+}
+
+// Values of up to 64 rows of one head, turned in LDS: a dim's tokens lie side by side in a page, so that 16 rows whose slots
+// follow one another from a multiple of 16 on leave as 16 bytes a dim; others byte by byte.  Column c of a dim is row
+// c - (first row's slot mod 16), which lines the runs up.
+__device__ __forceinline__ void values(const WriteArgs& a, int t0, int head) {
+  __shared__ uint8_t sm[128 * kPitch];
+  __shared__ int slots[kCols], whole[kCols / 16];
+  __shared__ size_t first[kCols];  // where the column's first dim lies in the cache
+  const int tid = threadIdx.x, j = tid & 7;
+  const int shift = max(slot_of(a, t0), 0) & 15;
+  int mine = -1;
+  if (tid < 128) {
+    mine = tid >= shift && tid < shift + kTokens ? slot_of(a, t0 + tid - shift) : -1;
+    const int blk = max(mine, 0) / a.BS;
+    if (tid < kCols) {
+      slots[tid] = mine;
+      first[tid] = ((size_t)blk * a.nkv + head) * 128 * a.BS + max(mine, 0) - blk * a.BS;
+    }
+    // sixteen columns that follow one another from a multiple of 16 on (as a page is one, they share it)
+    const int lead = __shfl(mine, tid & 48, 64);
+    const uint64_t run = __ballot(lead >= 0 && (lead & 15) == 0 && mine == lead + (tid & 15));
+    if (tid < kCols && (tid & 15) == 0) whole[tid >> 4] = ((run >> (tid & 63)) & 0xffff) == 0xffff;
+  }
+  u16x8 in[kTokens / 32][2];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) top = max(top, max(abs_bits(x[e]), abs_bits(y[e])));
+  for (int i = 0; i < kTokens / 32; ++i) {
+    const uint16_t* const p = a.qkv + (size_t)min(t0 + 32 * i + (tid >> 3), a.T - 1) * a.ld + (a.nq + a.nkv + head) * 128 + 8 * j;
+    in[i][0] = *reinterpret_cast<const u16x8*>(p);
+    in[i][1] = *reinterpret_cast<const u16x8*>(p + 64);
+  }
+  __syncthreads();
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-  const long slot = a.slots ? a.slots[t] : -1;
-  if (slot < 0 || slot >= a.cap) return;
-  const Step s = row_step(top);
-  const u32x2 q0 = pack8(x, s), q1 = pack8(y, s);
-  const bool key = h < a.nq + a.nkv;
-  const size_t page = (size_t)(slot / a.BS) * a.nkv + (h - a.nq - (key ? 0 : a.nkv));
-  const int off = (int)(slot % a.BS);
-  if (key) {
-    uint8_t* d = a.k + (page * a.BS + off) * 128 + 8 * j;
-    *reinterpret_cast<u32x2*>(d) = q0;
-    *reinterpret_cast<u32x2*>(d + 64) = q1;
-    if (j == 0) a.ks[page * a.BS + off] = s.scale;
-  } else {
-    uint8_t* d = a.v + (page * 128 + 8 * j) * (size_t)a.BS + off;
+  for (int i = 0; i < kTokens / 32; ++i) {
+    const int row = 32 * i + (tid >> 3);
+    float x[8], y[8];
+    uint32_t top = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      d[(size_t)e * a.BS] = (uint8_t)(q0[e >> 2] >> (8 * (e & 3)));
-      d[(size_t)(64 + e) * a.BS] = (uint8_t)(q1[e >> 2] >> (8 * (e & 3)));
+      x[e] = bf2f(in[i][0][e]), y[e] = bf2f(in[i][1][e]);
+      top = max(top, max(abs_bits(x[e]), abs_bits(y[e])));
     }
-    if (j == 0) a.vs[page * a.BS + off] = s.scale;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+    const Step s = row_step(top);
+    const u32x2 q0 = pack8(x, s), q1 = pack8(y, s);
+    uint8_t* const d = sm + 8 * j * kPitch + shift + row;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      d[e * kPitch] = (uint8_t)(q0[e >> 2] >> (8 * (e & 3)));
+      d[(64 + e) * kPitch] = (uint8_t)(q1[e >> 2] >> (8 * (e & 3)));
+    }
+    const int slot = slots[shift + row];
+    if (j == 0 && slot >= 0) {
+      const int blk = slot / a.BS;
+      a.vs[((size_t)blk * a.nkv + head) * a.BS + slot - blk * a.BS] = s.scale;
+    }
   }
+  __syncthreads();
+  for (int i = tid; i < 128 * (kCols / 16); i += 256) {
+    const int d = i / (kCols / 16), g = i % (kCols / 16);
+    if (whole[g]) {
+      const uint32_t* const p = reinterpret_cast<const uint32_t*>(sm + d * kPitch + 16 * g);
+      *reinterpret_cast<u32x4*>(a.v + first[16 * g] + (size_t)d * a.BS) = u32x4{p[0], p[1], p[2], p[3]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (slots[16 * g + e] >= 0) a.v[first[16 * g + e] + (size_t)d * a.BS] = sm[d * kPitch + 16 * g + e];
+    }
+  }
+}
+
+// TURN: the first v_blocks workgroups have the values, the others four tokens' rotations each.
+template <bool TURN>
+__global__ void __launch_bounds__(256) write_kernel(WriteArgs a, int v_blocks) {
+  const int b = blockIdx.x;
+  if constexpr (TURN)
+    if (b < v_blocks) return values(a, b / a.nkv * kTokens, b % a.nkv);
+  rotate<!TURN>(a, (b - v_blocks) * 4 + (threadIdx.x >> 6), threadIdx.x & 63);
 }
 
 }  // namespace q8
@@ -85,8 +185,11 @@ K8S_API int k8s_int8_write(void* qkv, long ld, const int* pos, const float* cos_
   if (T <= 0) return 0;
   if (nq < 0 || nkv <= 0 || BS <= 0 || max_pos <= 0) return (int)hipErrorInvalidValue;
   const WriteArgs a{(uint16_t*)qkv, ld, pos, cos_sin, slots, (uint8_t*)k, (uint8_t*)v, ks, vs, T, nq, nkv, BS, max_pos, cap};
-  const long blocks = ((long)T * (nq + 2 * nkv) * 8 + 255) / 256;
+  // The turn through LDS pays from a workgroup's rows on: us of 32 + 2 x 8 heads byte by byte / turned, 64 rows 9.1 / 8.8 (with 8.5 of the
+  // host), 1024 11.4 / 9.1, 8000 58 / 39; rows of as many pages 1024 18.6 / 17.7.
+  const bool turn = slots && T >= kTokens;
+  const long v_blocks = turn ? ((long)T + kTokens - 1) / kTokens * nkv : 0, blocks = v_blocks + ((long)T + 3) / 4;
   if (blocks > 0x7fffffffL) return (int)hipErrorInvalidValue;
-  hipLaunchKernelGGL(write_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL(turn ? write_kernel<true> : write_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a, (int)v_blocks);
   return (int)hipGetLastError();
 }
