@@ -21,7 +21,6 @@ forms below.  There are no gradients: under grad mode, inputs that ask for one a
 from __future__ import annotations
 
 import math
-from contextlib import nullcontext
 from dataclasses import dataclass
 from functools import lru_cache
 from typing import Optional, Tuple
@@ -29,7 +28,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import attention as A
-from ._lib import check, lib, ptr, stream_ptr, use_hip
+from ._lib import _raw_stream, check, lib, ptr
 
 HEAD_DIM = A.HEAD_DIM
 TINY = 2.0 ** -100
@@ -38,36 +37,45 @@ MAX_K = 131056
 _ROW_TYPES = (torch.bfloat16, torch.float32)
 
 
-def _inputs(t0: torch.Tensor, *more) -> None:
-    """One device for all; none that asks for a gradient."""
-    dev, grad = t0.device, torch.is_grad_enabled()
-    if grad and t0.requires_grad:
-        raise RuntimeError(_NO_GRADIENT)
-    for t in more:
-        if t is not None:
-            if t.device != dev:
-                raise ValueError(f"tensors on {dev} and {t.device}")
-            if grad and t.requires_grad:
-                raise RuntimeError(_NO_GRADIENT)
-
-
 _NO_GRADIENT = "the 8-bit operators have no gradients: detach the inputs or call under torch.no_grad()"
-_HERE = nullcontext()
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _on(t: torch.Tensor):
-    """The tensor's device as the current one while a kernel is launched."""
-    return _HERE if t.get_device() == _current_device() else torch.cuda.device(t.device)
+def _inputs(*tensors) -> int:
+    """One device for all, whose number this is (-1: the CPU); none that asks for a gradient."""
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors on {tensors[0].device} and {t.device}")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(_NO_GRADIENT)
+    return dev
 
 
-def _aligned(t: torch.Tensor) -> bool:
-    """Rows one behind another, each starting at a multiple of 16 bytes."""
-    return t.stride(1) == 1 and t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or t.stride(0) * t.element_size() % 16 == 0)
+def _call(name: str, dev: int, *args) -> None:
+    """The kernel's entry point on the current stream of device ``dev``, which is the current one meanwhile."""
+    fn = getattr(lib(), name)
+    if dev == _current_device():
+        check(fn(*args, _stream(dev)), name)
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, _stream(dev)), name)
 
 
-def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _stream(dev: int) -> int:
+    return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+
+
+def _pitch(t: torch.Tensor) -> int:
+    """Values from row to row of a matrix whose rows are dense and start at multiples of 16 bytes; 0 of another."""
+    (n, width), (ld, one) = t.shape, t.stride()
+    if (one != 1 and width > 1) or t.data_ptr() & 15:
+        return 0
+    if n <= 1:
+        return width
+    return 0 if ld * t.element_size() & 15 else ld
 
 
 def _quantised(y: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -83,16 +91,17 @@ def _quantised(y: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 # ------------------------------------------------------------------ rows
 def _rows(mode: int, x: torch.Tensor, H: int, out, scale, w=None, residual=None, eps: float = 0.0):
     T = x.shape[0]
-    _inputs(x, out, scale, w, residual)
-    dtype = x.dtype
+    dev, dtype = _inputs(x, out, scale, w, residual), x.dtype
     if dtype not in _ROW_TYPES:
         raise TypeError(f"rows must be bfloat16 or float32, not {dtype}")
     if H <= 0 or H % 16:
         raise ValueError(f"rows of a multiple of 16 values, not {H}")
     if out is None:
-        out = torch.empty((T, H), dtype=torch.int8, device=x.device)
-    elif out.dtype != torch.int8 or out.shape != (T, H) or not _aligned(out):
-        raise ValueError(f"out must be int8 {[T, H]} with 16-byte rows")
+        out, ldq = torch.empty((T, H), dtype=torch.int8, device=x.device), H
+    else:
+        ldq = _pitch(out) if out.dtype == torch.int8 and out.shape == (T, H) else 0
+        if not ldq:
+            raise ValueError(f"out must be int8 {[T, H]} with 16-byte rows")
     if scale is None:
         scale = torch.empty(T, dtype=torch.float32, device=x.device)
     elif scale.dtype != torch.float32 or scale.shape != (T,) or not scale.is_contiguous():
@@ -100,16 +109,17 @@ def _rows(mode: int, x: torch.Tensor, H: int, out, scale, w=None, residual=None,
     if w is not None and (w.dtype != dtype or w.shape != (H,)):
         raise ValueError(f"the norm's weight must be {dtype} {[H]}")
     if residual is not None and (residual.dtype != dtype or residual.shape != x.shape or not residual.is_contiguous()
-                                 or residual.data_ptr() % 16):
+                                 or residual.data_ptr() & 15):
         raise ValueError("the residual must be contiguous, 16-byte aligned and of the rows' shape and type")
-    if use_hip(x):
-        if not _aligned(x):
+    if dev >= 0:
+        ld = _pitch(x)
+        if not ld:
             x = x.clone(memory_format=torch.contiguous_format)
-        if w is not None and not (w.is_contiguous() and w.data_ptr() % 16 == 0):
+            ld = x.shape[1]
+        if w is not None and not (w.is_contiguous() and w.data_ptr() & 15 == 0):
             w = w.clone(memory_format=torch.contiguous_format)
-        with _on(x):
-            check(lib().k8s_int8_rows(mode, dtype == torch.float32, x.data_ptr(), _ld(x), ptr(residual), ptr(w), out.data_ptr(), _ld(out),
-                                      scale.data_ptr(), T, H, eps, stream_ptr(x)), "int8_rows")
+        _call("k8s_int8_rows", dev, mode, dtype is torch.float32, x.data_ptr(), ld, ptr(residual), ptr(w), out.data_ptr(), ldq,
+              scale.data_ptr(), T, H, eps)
         return out, scale
     y = x.float()
     if mode == 1:
@@ -170,9 +180,8 @@ def linear_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
     ``bias`` fp32 [N]; bf16 or fp32 out.  The integer sum is exact, so a row's result does not depend on the rows beside it."""
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
         raise ValueError(f"x [M, K] and w [N, K], not {list(x.shape)} and {list(w.shape)}")
-    M, K = x.shape
-    N = w.shape[0]
-    _inputs(x, x_scale, w, w_scale, bias, out)
+    (M, K), N = x.shape, w.shape[0]
+    dev = _inputs(x, x_scale, w, w_scale, bias, out)
     if x.dtype != torch.int8 or w.dtype != torch.int8:
         raise TypeError(f"x and w must be int8, not {x.dtype} and {w.dtype}")
     if not 0 < K <= MAX_K or K % 16:
@@ -183,22 +192,24 @@ def linear_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
     if out is None:
         if out_dtype not in _ROW_TYPES:
             raise TypeError(f"out_dtype must be bfloat16 or float32, not {out_dtype}")
-        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
-    elif out.dtype not in _ROW_TYPES or out.shape != (M, N) or out.stride(1) != 1:
-        raise ValueError(f"out must be bfloat16 or float32 {[M, N]}, its rows dense")
+        out, ldy = torch.empty((M, N), dtype=out_dtype, device=x.device), N
+    else:
+        if out.dtype not in _ROW_TYPES or out.shape != (M, N) or (out.stride(1) != 1 and N > 1):
+            raise ValueError(f"out must be bfloat16 or float32 {[M, N]}, its rows dense")
+        ldy = out.stride(0) if M > 1 else N
     if M == 0 or N == 0:
         return out
-    if use_hip(x):
-        if not _aligned(x):
+    if dev >= 0:
+        ldx, ldw = _pitch(x), _pitch(w)
+        if not ldx:
             x = x.clone(memory_format=torch.contiguous_format)
-        if not _aligned(w):
+            ldx = K
+        if not ldw:
             raise ValueError("w's rows must be dense and start at multiples of 16 bytes")
         kind, runs, n = product_plan(M, N, K)
-        with _on(x):
-            part = torch.empty(n, dtype=torch.int32, device=x.device) if n else None
-            check(lib().k8s_int8_gemm(x.data_ptr(), _ld(x), x_scale.data_ptr(), w.data_ptr(), _ld(w), w_scale.data_ptr(), ptr(bias),
-                                      out.data_ptr(), _ld(out), out.dtype == torch.float32, M, N, K, kind, runs, ptr(part), n,
-                                      stream_ptr(x)), "int8_gemm")
+        part = torch.empty(n, dtype=torch.int32, device=x.device) if n else None
+        _call("k8s_int8_gemm", dev, x.data_ptr(), ldx, x_scale.data_ptr(), w.data_ptr(), ldw, w_scale.data_ptr(), ptr(bias),
+              out.data_ptr(), ldy, out.dtype is torch.float32, M, N, K, kind, runs, ptr(part), n)
         return out
     # (in fp64 every partial sum is an integer below 2^53: exact)
     y = (x.double() @ w.double().T).float() * x_scale[:, None] * w_scale
@@ -257,7 +268,7 @@ def rope_kv_write_int8(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torc
     ``attention.rope_kv_write``, the rows of one call have different slots."""
     T = qkv.shape[0]
     _heads(qkv, cache, nq, nkv, (nq + 2 * nkv) * HEAD_DIM, "qkv")
-    _inputs(qkv, positions, cos_sin, slots, cache.k)
+    dev = _inputs(qkv, positions, cos_sin, slots, cache.k)
     for t in (positions, slots):
         if t is not None and (t.dtype != torch.int32 or t.shape != (T,) or not t.is_contiguous()):
             raise ValueError(f"positions and slots must be contiguous int32 {[T]}, not {t.dtype} {list(t.shape)}")
@@ -266,13 +277,12 @@ def rope_kv_write_int8(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torc
     NB, _, BS, D = cache.k.shape
     if T == 0:
         return
-    if use_hip(qkv):
-        if not _aligned(qkv) or cos_sin.data_ptr() % 16:
+    if dev >= 0:
+        ld = _pitch(qkv)
+        if not ld or cos_sin.data_ptr() & 15:
             raise ValueError("the rows of qkv and cos_sin must be dense and start at multiples of 16 bytes")
-        with _on(qkv):
-            check(lib().k8s_int8_write(qkv.data_ptr(), _ld(qkv), positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], ptr(slots),
-                                       cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), T, nq, nkv,
-                                       BS, NB * BS, stream_ptr(qkv)), "int8_write")
+        _call("k8s_int8_write", dev, qkv.data_ptr(), ld, positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], ptr(slots),
+              cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), T, nq, nkv, BS, NB * BS)
         return
     nh = nq + nkv
     cos, sin = cos_sin[positions.long().clamp(0, cos_sin.shape[0] - 1)][:, None].chunk(2, -1)
@@ -300,23 +310,26 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
     _heads(q, cache, nq, nkv, nq * HEAD_DIM, "q")
     NB, _, BS, D = cache.k.shape
     S, bt, ctx, starts = meta.num_seqs, meta.block_tables, meta.ctx_lens, meta.q_start
-    _inputs(q, bt, ctx, starts, cache.k, out)
+    dev = _inputs(q, bt, ctx, starts, cache.k, out)
     if out is None:
-        out = torch.empty((T, nq * D), dtype=q.dtype, device=q.device)
-    elif out.shape != (T, nq * D) or out.dtype != q.dtype or out.stride(1) != 1:
-        raise ValueError("out must be [T, nq 128] of q's type, its rows dense")
+        out, ldo = torch.empty((T, nq * D), dtype=q.dtype, device=q.device), nq * D
+    else:
+        if out.shape != (T, nq * D) or out.dtype != q.dtype or out.stride(1) != 1:
+            raise ValueError("out must be [T, nq 128] of q's type, its rows dense")
+        ldo = out.stride(0) if T > 1 else nq * D
     if T == 0 or S == 0:
         return out
-    if not use_hip(q):
+    if dev < 0:
         return _attention_plain(q, cache, meta, nq, nkv, scale, out)
     if bt.dtype != torch.int32 or bt.dim() != 2 or bt.shape[0] < S or bt.stride(1) != 1:
         raise ValueError("block_tables must be int32 [S, pages]")
     if ctx.dtype != torch.int32 or starts.dtype != torch.int32 or ctx.numel() < S or starts.numel() < S + 1:
         raise ValueError("ctx_lens must be int32 [S] and q_start int32 [S + 1]")
-    if not _aligned(q):
+    ldq = _pitch(q)
+    if not ldq:
         raise ValueError("q's rows must be dense and start at multiples of 16 bytes")
-    G, L = nq // nkv, lib()
-    common = (q.data_ptr(), _ld(q), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), NB,
+    G = nq // nkv
+    common = (q.data_ptr(), ldq, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), NB,
               bt.data_ptr(), bt.stride(0) if S > 1 else bt.shape[1], ctx.data_ptr(), starts.data_ptr())
     if meta.decode:
         if T != S:
@@ -328,10 +341,8 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
         if meta.n_parts > 1 and meta.part_o is None:
             raise ValueError("a plan of several parts needs part_o and part_ml")
         grid = max(1, meta.grid_waves or min(A.DECODE_WAVE_SLOTS, meta.n_items * nkv))
-        with _on(q):
-            check(L.k8s_int8_attn_reply(*common, S, nq, nkv, BS, scale, out.data_ptr(), _ld(out), ptr(meta.part_o), ptr(meta.part_ml),
-                                        meta.n_parts, meta.part_size, meta.items.data_ptr(), meta.n_items, ptr(meta.d_n_items), grid,
-                                        stream_ptr(q)), "int8_attn_reply")
+        _call("k8s_int8_attn_reply", dev, *common, S, nq, nkv, BS, scale, out.data_ptr(), ldo, ptr(meta.part_o), ptr(meta.part_ml),
+              meta.n_parts, meta.part_size, meta.items.data_ptr(), meta.n_items, ptr(meta.d_n_items), grid)
         return out
     rows = A.prefill_tile_tokens(G, BS) * G
     if rows > A.PF8_ROWS:
@@ -340,11 +351,9 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
         raise ValueError("the step has no plan: attach_plan")
     if meta.n_merge and meta.pf_o is None:
         meta.pf_o, meta.pf_ml = A.prefill_workspace(nkv, q.device, max(meta.m_slot0_end(), 1))
-    with _on(q):
-        check(L.k8s_int8_attn_chunk(*common, nq, nkv, BS, scale, out.data_ptr(), _ld(out), ptr(meta.tile_seq), ptr(meta.tile_tok0),
-                                    ptr(meta.tile_len), ptr(meta.tile_kv0), ptr(meta.tile_kv1), ptr(meta.tile_slot), meta.n_tiles, rows,
-                                    ptr(meta.m_tok0), ptr(meta.m_len), ptr(meta.m_slot0), ptr(meta.m_np), meta.n_merge, ptr(meta.pf_o),
-                                    ptr(meta.pf_ml), A.PF8_ROWS, stream_ptr(q)), "int8_attn_chunk")
+    _call("k8s_int8_attn_chunk", dev, *common, nq, nkv, BS, scale, out.data_ptr(), ldo, ptr(meta.tile_seq), ptr(meta.tile_tok0),
+          ptr(meta.tile_len), ptr(meta.tile_kv0), ptr(meta.tile_kv1), ptr(meta.tile_slot), meta.n_tiles, rows, ptr(meta.m_tok0),
+          ptr(meta.m_len), ptr(meta.m_slot0), ptr(meta.m_np), meta.n_merge, ptr(meta.pf_o), ptr(meta.pf_ml), A.PF8_ROWS)
     return out
 
 
