@@ -28,7 +28,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import attention as A
-from ._lib import _raw_stream, check, lib, ptr
+from ._lib import _raw_stream, check, lib, ptr, scratch
 
 HEAD_DIM = A.HEAD_DIM
 TINY = 2.0 ** -100
@@ -264,8 +264,8 @@ def rope_kv_write_int8(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torc
                        nq: int, nkv: int) -> None:
     """Rotate the q heads of ``qkv`` [T, >= (nq + 2 nkv) 128] in place and write its keys (rotated, quantised from fp32) and
     values to the cache's slots.  The k and v columns stay as they came.  A row whose slot is negative (all rows, where
-    ``slots`` is None) is rotated and not kept; nor is one whose slot the pool does not have.  As in
-    ``attention.rope_kv_write``, the rows of one call have different slots."""
+    ``slots`` is None) is rotated and not kept; nor is one whose slot the pool does not have.  A position outside ``cos_sin``
+    takes its nearest row.  As in ``attention.rope_kv_write``, the rows of one call have different slots."""
     T = qkv.shape[0]
     _heads(qkv, cache, nq, nkv, (nq + 2 * nkv) * HEAD_DIM, "qkv")
     dev = _inputs(qkv, positions, cos_sin, slots, cache.k)
@@ -349,11 +349,13 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
         raise ValueError(f"{G} query heads a key head: a tile takes {A.PF8_ROWS}")
     if meta.tile_seq is None or meta.tile_kv1 is None:
         raise ValueError("the step has no plan: attach_plan")
-    if meta.n_merge and meta.pf_o is None:
-        meta.pf_o, meta.pf_ml = A.prefill_workspace(nkv, q.device, max(meta.m_slot0_end(), 1))
+    part_o, part_ml = meta.pf_o, meta.pf_ml
+    if meta.n_merge and part_o is None:  # (a split tile's parts are tiles of the plan: no more than those, without a look at the device)
+        part_o = scratch(meta.n_tiles * nkv * A.PF8_ROWS * D, torch.float32, q.device)
+        part_ml = scratch(meta.n_tiles * nkv * A.PF8_ROWS * 2, torch.float32, q.device)
     _call("k8s_int8_attn_chunk", dev, *common, nq, nkv, BS, scale, out.data_ptr(), ldo, ptr(meta.tile_seq), ptr(meta.tile_tok0),
           ptr(meta.tile_len), ptr(meta.tile_kv0), ptr(meta.tile_kv1), ptr(meta.tile_slot), meta.n_tiles, rows, ptr(meta.m_tok0),
-          ptr(meta.m_len), ptr(meta.m_slot0), ptr(meta.m_np), meta.n_merge, ptr(meta.pf_o), ptr(meta.pf_ml), A.PF8_ROWS)
+          ptr(meta.m_len), ptr(meta.m_slot0), ptr(meta.m_np), meta.n_merge, ptr(part_o), ptr(part_ml), A.PF8_ROWS)
     return out
 
 

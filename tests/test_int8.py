@@ -413,6 +413,72 @@ def test_reply(device, lens, nq, nkv, BS, part):
     assert bool((out[:, nq * D:] == 7).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,nkv", [(8, 2), (16, 1), (8, 8)])
+@pytest.mark.parametrize("part", [64, 256, 2048])
+def test_reply_rows_that_share_a_sequence(nq, nkv, part):
+    """Consecutive tokens of one sequence as rows of a reply step share their keys' reads: as many as the 16 rows of a wave hold."""
+    q, cache, meta, starts, ctx = attn_case("cuda", [(1, 700), (1, 70), (1, 300)], nq, nkv)
+    rows = [(0, 694 + i) for i in range(7)] + [(1, 70)] + [(2, 299), (2, 300)]
+    q = randn(gen(5), len(rows), nq * D, dtype=BF, device="cuda")
+    bt = meta.block_tables[[s for s, _ in rows]].contiguous()
+    lens = [c for _, c in rows]
+    meta = A.AttnMeta(block_tables=bt, ctx_lens=torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                      q_start=torch.arange(len(rows) + 1, dtype=torch.int32, device="cuda"), num_seqs=len(rows), decode=True)
+    chain = [i > 0 and rows[i][0] == rows[i - 1][0] for i in range(len(rows))]
+    A.attach_decode_plan(meta, lens, nq, nkv, 64, "cuda", part=part, chain=chain)
+    assert meta.n_items < sum(-(-c // part) for c in lens) or nq // nkv == 16
+    out = Q.paged_attention_int8(q, cache, meta, nq, nkv, 0.09)
+    check_attention(out, q, cache, meta, list(range(len(rows) + 1)), lens, nq, nkv, 0.09)
+
+
+@pytest.mark.gpu
+def test_reply_plan_read_on_the_device():
+    """A captured step reads its list's length and its parts' size when it is replayed, and grows and shrinks with them."""
+    nq, nkv = 8, 2
+    q, cache, meta, starts, ctx = attn_case("cuda", [(1, 900), (1, 900), (1, 900)], nq, nkv)
+    room = torch.zeros(64, 4, dtype=torch.int32, device="cuda")
+    meta.items, meta.n_items, meta.d_n_items = room, 64, torch.zeros(2, dtype=torch.int32, device="cuda")
+    meta.n_parts, meta.part_size, meta.grid_waves = 16, 64, 40
+    meta.part_o = torch.empty(3 * nq * 16 * D, device="cuda")
+    meta.part_ml = torch.empty(3 * nq * 16 * 2, device="cuda")
+
+    def plan(lens, part):
+        items = torch.from_numpy(A.build_decode_items(lens, range(3), part)).cuda()
+        room[:len(items)] = items
+        meta.d_n_items.copy_(torch.tensor([len(items), part], dtype=torch.int32))
+        meta.ctx_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+
+    plan([900, 900, 900], 64)
+    Q.paged_attention_int8(q, cache, meta, nq, nkv, 0.09)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = Q.paged_attention_int8(q, cache, meta, nq, nkv, 0.09)
+    for lens, part in (([900, 900, 900], 64), ([900, 1, 65], 320), ([0, 128, 512], 64), ([900, 800, 0], 1024), ([64, 65, 900], 64)):
+        plan(lens, part)
+        graph.replay()
+        torch.cuda.synchronize()
+        check_attention(out, q, cache, meta, [0, 1, 2, 3], lens, nq, nkv, 0.09)
+
+
+@pytest.mark.gpu
+def test_a_split_chunk_is_captured_without_a_run_before():
+    q, cache, meta, starts, ctx = attn_case("cuda", [(70, 3000)], 8, 2)
+    planned(meta, starts, ctx, 8, 2, 64)
+    assert meta.n_merge
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = Q.paged_attention_int8(q, cache, meta, 8, 2, 0.09)
+    want = Q.paged_attention_int8(q, cache, meta, 8, 2, 0.09)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    check_attention(out, q, cache, meta, starts, ctx, 8, 2, 0.09)
+
+
 CHUNKS = [
     ([(2, 2)], 4, 1, 64), ([(5, 5), (1, 70), (64, 64), (3, 200)], 8, 2, 64), ([(130, 700), (1, 1), (65, 65)], 32, 8, 64),
     ([(100, 100)], 8, 8, 128), ([(300, 1500)], 16, 1, 64), ([(0, 90), (17, 130), (0, 0), (2, 64)], 12, 4, 192),
