@@ -3,6 +3,8 @@
 //
 // The matrix instruction is v_mfma_i32_16x16x64_i8 with the weight as its first operand: lane l holds 16 bytes of row l & 15
 // at byte 16 (l >> 4), and gets the sums of columns 4 (l >> 4) .. + 3 of row l & 15 of x, so that it stores four neighbours.
+#include <cmath>
+
 #include "int8_rows.h"
 
 namespace k8s {
@@ -124,7 +126,10 @@ __global__ void __launch_bounds__(64 * kWaves) few_kernel(GemmArgs a) {
 // A stage holds rows of 128 bytes of K: 16-byte piece c of row r at c ^ ((r >> 1) & 7), so that the 16 lanes of a fragment's
 // read hit 16 different bank groups.  The DMA writes LDS in lane order, so that the exchange is in its source address.
 typedef __attribute__((address_space(3))) void lds_t;
-__device__ __forceinline__ void dma16(const uint8_t* src, uint8_t* dst) { __builtin_amdgcn_global_load_lds(src, (lds_t*)dst, 16, 0, 0); }
+template <int POLICY = 0>  // 2: non-temporal
+__device__ __forceinline__ void dma16(const uint8_t* src, uint8_t* dst) {
+  __builtin_amdgcn_global_load_lds(src, (lds_t*)dst, 16, 0, POLICY);
+}
 __device__ __forceinline__ void bar() {
   __builtin_amdgcn_sched_barrier(0);
   __builtin_amdgcn_s_barrier();
@@ -161,6 +166,9 @@ __global__ void __launch_bounds__(128 * WN, 2) ring_kernel(GemmArgs a, int n_mt,
   tile_at(t0 / a.splits, n_mt, n_nt, tm, tn);
   const int m0 = tm * BM, n0 = tn * BN;
   const int all = (a.K + 127) >> 7, per = (all + a.splits - 1) / a.splits, kt0 = slice * per, nt = min(all - kt0, per);
+  // One row of tiles over an uncut K streams the weight by, and it need not stay in the caches: 17 and 48 rows of 128256 x 4096 99 -> 92
+  // and 112 -> 108 us, of 28672 x 4096 26.8 -> 25.0 and 29.7 -> 28.2 (with K in four runs 4096 x 14336 took longer: 16.4 -> 17.9).
+  const bool once = n_mt == 1 && a.splits == 1;
 
   const uint8_t* src[I];
   int lch[I];
@@ -176,7 +184,11 @@ __global__ void __launch_bounds__(128 * WN, 2) ring_kernel(GemmArgs a, int n_mt,
     for (int i = 0; i < I; ++i) {
       // (zeros behind K: in both operands, since both may be rows of one tensor that goes on)
       const uint8_t* p = k + lch[i] < a.K ? src[i] + k + lch[i] : reinterpret_cast<const uint8_t*>(&kZeros);
-      dma16(p, sm + stage * STAGE + (I * wv + i) * 1024);
+      uint8_t* const to = sm + stage * STAGE + (I * wv + i) * 1024;
+      if (once && 8 * (I * wv + i) >= BM)
+        dma16<2>(p, to);
+      else
+        dma16(p, to);
     }
   };
   const int r = lane & 15, g = lane >> 4;
@@ -380,37 +392,39 @@ __global__ void __launch_bounds__(256) join_big_kernel(GemmArgs a, int n_mt, int
 // Rows and columns of a tile by kind.
 constexpr int kEdge[7][2] = {{16, 16}, {32, 64}, {64, 64}, {64, 128}, {128, 64}, {128, 128}, {256, 256}};
 
-// Estimated us of a product.  The tiles' time is rounds over the 256 compute units, each `stages` of 128 bytes of K and a fixed part;
-// the middle tiles lie two on a unit, where a stage takes longer.  A product takes no less than its weight's way from memory.
-// Few rows: the weight's way and the rows' reads beside it, or the latency of each wave's turns over K (four steps of 64 bytes
-// a turn), and what a workgroup costs beside its loads, which shows where K is short.  The constants are a fit to times of every kind
-// and cut at 360 sizes from 1 to 5000 rows, 512 to 128256 columns and K from 512 to 28672, the weights from memory: the choice is
-// 1 % from the best one on average.
+// Estimated us of a product.  Its tiles take rounds over the 256 compute units, a round `per` stages of 128 bytes of K and a fixed part;
+// the middle tiles lie two on a unit, where a stage takes longer.  Beside that stands the weight's way from memory: the third
+// root of the cubes' sum, roughly, since the one hides in the other until they are alike.  Few rows: the weight's way with the
+// rows' reads beside it, against the latency of each wave's turns over K (four steps of 64 bytes a turn), and what a workgroup
+// costs beside its loads, which shows where K is short.  The constants are a fit to times of every kind and cut at 480 sizes: 1 to
+// 4096 rows by 16 weights of 512 x 512 to 128256 x 4096 (K from 512 to 28672), the weights from memory.  The choice is 1.3 % from
+// the best one on average; furthest off are 13 and 16 rows of 5120 x 5120, 14.6 and 16.0 us for 10.9.
 inline double cost(int M, int N, int K, int kind, int splits) {
-  constexpr double kStart = 2.25, kByte = 0.172e-6, kJoin = 2.47, kJoinByte = 0.352e-6;
-  // us a stage alone on a unit, by twos (256 x 256: with few units busy), a round's fixed part
-  constexpr double c[7][3] = {{}, {.216, .425, 1.84}, {.272, .526, 1.64}, {.432, .860, 1.53}, {.472, .760, 1.83}, {.623, .466, 2.43}, {1.55, 1.01, 5.11}};
+  constexpr double kStart = 2.62, kByte = 0.150e-6, kJoin = 2.46, kJoinByte = 0.328e-6;
+  // us a stage alone on a unit, by twos (of the two largest: with few units busy), a round's fixed part
+  constexpr double c[7][3] = {{}, {.260, .434, 1.54}, {.361, .525, 1.44}, {.453, .809, 1.60}, {.592, .800, 2.00}, {.643, .542, 2.61}, {1.44, .995, 5.61}};
   const double bytes = (double)N * K;
   if (kind == 0) {
-    const double turns = (K + 64 * kWaves * 4 - 1) / (64 * kWaves * 4), stream = bytes * (0.163e-6 + 0.0057e-6 * (M - 1));
-    const double wait = turns * (1.13 + 0.04 * (M - 1));
-    return kStart + (wait > stream ? wait : stream) + 0.0025 * ((N + 15) / 16) * (K > 1024 ? 1024. / K : 1.);
+    const double turns = (K + 64 * kWaves * 4 - 1) / (64 * kWaves * 4), stream = bytes * (0.168e-6 + 0.00664e-6 * (M - 1));
+    const double wait = turns * (1.04 + 0.0501 * (M - 1));
+    return kStart + pow(pow(stream, 4.09) + pow(wait, 4.09), 1 / 4.09) + 0.00247 * ((N + 15) / 16) * (K > 1024 ? 1024. / K : 1.);
   }
   const int stages = (K + 127) / 128, per = (stages + splits - 1) / splits;
   const long tiles = (long)((M - 1) / kEdge[kind][0] + 1) * ((N - 1) / kEdge[kind][1] + 1);
   const double a = c[kind][0], b = c[kind][1], e = c[kind][2];
-  double t, joined;
-  if (kind >= 5) {
-    const long whole = kind == 6 ? tiles / 256 : tiles * splits / 256, rest = kind == 6 ? tiles % 256 * splits : tiles * splits % 256;
-    t = whole * ((kind == 6 ? stages : per) * a + e) + (rest ? per * (b + (a - b) * rest / 256.) + e : 0);
-    joined = kind == 6 ? 65536. * rest : (double)splits * M * N;
+  double t, joined = (double)splits * M * N;
+  if (kind == 6) {
+    const long whole = tiles / 256, rest = tiles % 256 * splits;
+    t = whole * (stages * a + e) + (rest ? per * (b + (a - b) * rest / 256.) + e : 0);
+    joined = 65536. * rest;
+  } else if (kind == 5) {
+    const long whole = tiles * splits / 256, rest = tiles * splits % 256;
+    t = whole * (per * a + e) + (rest ? per * (b + (a - b) * rest / 256.) + e : 0);
   } else {
     const long whole = tiles * splits / 512, rest = tiles * splits % 512;
     t = whole * (per * b + e) + (rest ? per * (rest > 256 ? b : a) + e : 0);
-    joined = (double)splits * M * N;
   }
-  if (t < bytes * kByte + 2 * e) t = bytes * kByte + 2 * e;
-  return kStart + t + (splits > 1 ? kJoin + kJoinByte * 4 * joined : 0);
+  return kStart + pow(pow(t, 2.82) + pow(bytes * kByte, 2.82), 1 / 2.82) + (splits > 1 ? kJoin + kJoinByte * 4 * joined : 0);
 }
 // Whether `splits` runs of K are possible: none of them empty, and of 256 x 256 tiles only as many as the rest of a round holds.
 inline bool can_cut(int M, int N, int K, int kind, int splits) {
