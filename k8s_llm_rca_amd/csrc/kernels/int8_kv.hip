@@ -27,10 +27,11 @@ __device__ __forceinline__ int slot_of(const WriteArgs& a, int t) {
   return s < a.cap ? s : -1;
 }
 
-// A wave a token, eight lanes a head (lane j has dims 8j .. 8j+7 and their partners 64 on), so that a lane reads its cosines
-// once for all heads.  VALUES: the value heads, too, byte by byte.
+// Eight lanes a head (lane j has dims 8j .. 8j+7 and their partners 64 on), which read their cosines once for all heads that they
+// take; a token's heads go by eights to `parts` waves in turn, of which this is wave `part`.  VALUES: the value heads, too,
+// byte by byte.
 template <bool VALUES>
-__device__ __forceinline__ void rotate(const WriteArgs& a, int t, int lane) {
+__device__ __forceinline__ void rotate(const WriteArgs& a, int t, int part, int parts, int lane) {
   if (t >= a.T) return;
   const int j = lane & 7, heads = a.nq + (VALUES ? 2 : 1) * a.nkv;
   uint16_t* const row = a.qkv + (size_t)t * a.ld + 8 * j;
@@ -44,17 +45,17 @@ __device__ __forceinline__ void rotate(const WriteArgs& a, int t, int lane) {
     si[e] = *reinterpret_cast<const f32x4*>(cs + 64 + 4 * e);
   }
   constexpr int U = 5;
-  for (int h0 = lane >> 3; h0 < heads; h0 += 8 * U) {
+  for (int h0 = 8 * part + (lane >> 3); h0 < heads; h0 += 8 * U * parts) {
     u16x8 lo[U], hi[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint16_t* const p = row + min(h0 + 8 * u, heads - 1) * 128;
+      const uint16_t* const p = row + min(h0 + 8 * u * parts, heads - 1) * 128;
       lo[u] = *reinterpret_cast<const u16x8*>(p);
       hi[u] = *reinterpret_cast<const u16x8*>(p + 64);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int h = h0 + 8 * u;
+      const int h = h0 + 8 * u * parts;
       if (h >= heads) break;
       float x[8], y[8];
       const bool turned = !VALUES || h < a.nq + a.nkv;
@@ -104,6 +105,13 @@ __device__ __forceinline__ void values(const WriteArgs& a, int t0, int head) {
   __shared__ int slots[kCols], whole[kCols / 16];
   __shared__ size_t first[kCols];  // where the column's first dim lies in the cache
   const int tid = threadIdx.x, j = tid & 7;
+  u16x8 in[kTokens / 32][2];
+#pragma unroll
+  for (int i = 0; i < kTokens / 32; ++i) {
+    const uint16_t* const p = a.qkv + (size_t)min(t0 + 32 * i + (tid >> 3), a.T - 1) * a.ld + (a.nq + a.nkv + head) * 128 + 8 * j;
+    in[i][0] = *reinterpret_cast<const u16x8*>(p);
+    in[i][1] = *reinterpret_cast<const u16x8*>(p + 64);
+  }
   const int shift = max(slot_of(a, t0), 0) & 15;
   int mine = -1;
   if (tid < 128) {
@@ -117,13 +125,6 @@ __device__ __forceinline__ void values(const WriteArgs& a, int t0, int head) {
     const int lead = __shfl(mine, tid & 48, 64);
     const uint64_t run = __ballot(lead >= 0 && (lead & 15) == 0 && mine == lead + (tid & 15));
     if (tid < kCols && (tid & 15) == 0) whole[tid >> 4] = ((run >> (tid & 63)) & 0xffff) == 0xffff;
-  }
-  u16x8 in[kTokens / 32][2];
-#pragma unroll
-  for (int i = 0; i < kTokens / 32; ++i) {
-    const uint16_t* const p = a.qkv + (size_t)min(t0 + 32 * i + (tid >> 3), a.T - 1) * a.ld + (a.nq + a.nkv + head) * 128 + 8 * j;
-    in[i][0] = *reinterpret_cast<const u16x8*>(p);
-    in[i][1] = *reinterpret_cast<const u16x8*>(p + 64);
   }
   __syncthreads();
 #pragma unroll
@@ -166,13 +167,14 @@ __device__ __forceinline__ void values(const WriteArgs& a, int t0, int head) {
   }
 }
 
-// TURN: the first v_blocks workgroups have the values, the others four tokens' rotations each.
+// TURN: the first v_blocks workgroups have the values, the others four waves of rotations each.
 template <bool TURN>
-__global__ void __launch_bounds__(256) write_kernel(WriteArgs a, int v_blocks) {
+__global__ void __launch_bounds__(256) write_kernel(WriteArgs a, int v_blocks, int parts) {
   const int b = blockIdx.x;
   if constexpr (TURN)
     if (b < v_blocks) return values(a, b / a.nkv * kTokens, b % a.nkv);
-  rotate<!TURN>(a, (b - v_blocks) * 4 + (threadIdx.x >> 6), threadIdx.x & 63);
+  const int w = (b - v_blocks) * 4 + (threadIdx.x >> 6);
+  rotate<!TURN>(a, w / parts, w % parts, parts, threadIdx.x & 63);
 }
 
 }  // namespace q8
@@ -185,11 +187,15 @@ K8S_API int k8s_int8_write(void* qkv, long ld, const int* pos, const float* cos_
   if (T <= 0) return 0;
   if (nq < 0 || nkv <= 0 || BS <= 0 || max_pos <= 0) return (int)hipErrorInvalidValue;
   const WriteArgs a{(uint16_t*)qkv, ld, pos, cos_sin, slots, (uint8_t*)k, (uint8_t*)v, ks, vs, T, nq, nkv, BS, max_pos, cap};
-  // The turn through LDS pays from a workgroup's rows on: us of 32 + 2 x 8 heads byte by byte / turned, 64 rows 9.1 / 8.8 (with 8.5 of the
-  // host), 1024 11.4 / 9.1, 8000 58 / 39; rows of as many pages 1024 18.6 / 17.7.
-  const bool turn = slots && T >= kTokens;
-  const long v_blocks = turn ? ((long)T + kTokens - 1) / kTokens * nkv : 0, blocks = v_blocks + ((long)T + 3) / 4;
+  // The turn through LDS pays from some tokens and heads on.  us byte by byte / turned, rows whose slots follow one another: 32 + 2 x 8
+  // heads at 512 rows 7.0 / 8.5, 768 9.3 / 8.7, 8000 58.6 / 40.1; 8 + 2 x 1 heads at 4096 rows 8.1 / 9.2, 6000 10.6 / 10.1; 16 + 2 x
+  // 16 heads at 256 rows 7.3 / 8.1, 512 9.9 / 8.4.  Slots in as many pages: 32 + 2 x 8 heads at 1024 rows 18.5 / 17.7.
+  const bool turn = slots && (long)T * nkv >= 6000;
+  // few tokens: a wave eight heads, so that no wave takes them one after another (one row of 32 + 2 x 8 heads 4.8 -> 3.3 us, 128 rows
+  // 7.0 -> 4.2)
+  const int eights = (nq + (turn || !slots ? 1 : 2) * nkv + 7) / 8, parts = T >= 2048 ? 1 : T * eights <= 2048 ? eights : 2048 / T;
+  const long v_blocks = turn ? ((long)T + kTokens - 1) / kTokens * nkv : 0, blocks = v_blocks + ((long)T * parts + 3) / 4;
   if (blocks > 0x7fffffffL) return (int)hipErrorInvalidValue;
-  hipLaunchKernelGGL(turn ? write_kernel<true> : write_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a, (int)v_blocks);
+  hipLaunchKernelGGL(turn ? write_kernel<true> : write_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a, (int)v_blocks, parts);
   return (int)hipGetLastError();
 }

@@ -160,16 +160,23 @@ __global__ void __launch_bounds__(W >= 4 ? 64 * W : 256) rows_kernel(RowArgs a) 
   }
 }
 
+// Waves a row.  Few rows wait for their own loads and exchange: a piece a lane, two at most.  Many rows fill the chip by themselves:
+// fewer waves a row, up to four pieces a lane.  us of a norm with its residual, bf16, at 32 / 8192 rows: 1024 wide by 1 wave
+// 3.7 / 10.0, by 4 3.2 / 16.0; 2048 wide by 1 4.7 / 19.7, by 4 3.2 / 22.2; 4096 wide by 4 3.8 / 37.0, by 8 3.3 / 38.4; 8192 wide by 4
+// 4.9 / 77.8, by 8 3.9 / 77.2, by 16 3.9 / 82.1; 14336 wide by 8 4.8 / 156, by 16 4.5 / 152.
 template <int MODE, typename E>
 int launch(const RowArgs& a, hipStream_t st) {
   const int nv = a.H >> 3;
-  if (nv <= 256)  // up to 2048 wide: a wave a row
+  const bool many = a.T > 1024;
+  if (nv <= (many ? 256 : 64))
     hipLaunchKernelGGL((rows_kernel<MODE, E, 1, 4>), dim3((a.T + 3) / 4), dim3(256), 0, st, a);
-  else if (nv <= 1024)
+  else if (nv <= (many ? 512 : 256))
     hipLaunchKernelGGL((rows_kernel<MODE, E, 4, 4>), dim3(a.T), dim3(256), 0, st, a);
+  else if (nv <= 1024)
+    hipLaunchKernelGGL((rows_kernel<MODE, E, 8, 4>), dim3(a.T), dim3(512), 0, st, a);
   else if (nv <= 4096)
     hipLaunchKernelGGL((rows_kernel<MODE, E, 16, 4>), dim3(a.T), dim3(1024), 0, st, a);
-  else
+  else  // (over 32768 wide: the row is read twice)
     hipLaunchKernelGGL((rows_kernel<MODE, E, 16, 0>), dim3(a.T), dim3(1024), 0, st, a);
   return (int)hipGetLastError();
 }

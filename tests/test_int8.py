@@ -91,6 +91,21 @@ def test_norm(device, dtype, residual, T, H):
     check_rows(q, s, y, 2.0 ** -22, 2.0 ** -17)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1024, 1025])
+@pytest.mark.parametrize("H", [512, 528, 2048, 2064, 4096, 4112])
+def test_many_rows(T, H):
+    """Both sides of where a row's waves change."""
+    g = gen(T + H)
+    x, r, w = randn(g, T, H, dtype=BF), randn(g, T, H, dtype=BF), (1 + 0.1 * randn(g, H)).to(BF)
+    check_rows(*Q.quantize_rows(x.cuda()), x, 2.0 ** -24)
+    h = (x.float() + r.float()).to(BF).double()
+    rd = r.cuda()
+    q, s = Q.rmsnorm_int8(x.cuda(), w.cuda(), 1e-5, residual=rd)
+    assert torch.equal(rd.cpu().double(), h)
+    check_rows(q, s, h * w.double() / (h.square().mean(-1, keepdim=True) + 1e-5).sqrt(), 2.0 ** -22, 2.0 ** -17)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("H", [128, 4096, 16384, 33008])
 def test_rows_that_hold_no_number(device, H):
