@@ -17,22 +17,23 @@ constexpr float kTiny = 0x1p-100f;
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 struct Step {
-  float inv;    // integers a unit of y
-  float scale;  // what an integer stands for; NaN where the row holds a NaN or an infinity (its integers are zeros)
+  float inv, rest;  // integers a unit of y, and what rounding it left
+  float scale;      // what an integer stands for; NaN where the row holds a NaN or an infinity (its integers are zeros)
 };
 __device__ __forceinline__ Step row_step(uint32_t top) {
   const float t = __uint_as_float(top);
-  if (top >= 0x7f800000u) return {0.f, __uint_as_float(0x7fc00000u)};
-  if (t < kTiny) return {0.f, 0.f};
-  return {127.f / t, t / 127.f};
+  if (top >= 0x7f800000u) return {0.f, 0.f, __uint_as_float(0x7fc00000u)};
+  if (t < kTiny) return {0.f, 0.f, 0.f};
+  const float inv = 127.f / t;
+  return {inv, fmaf(-inv, t, 127.f) / t, t / 127.f};
 }
 
-// y inv to the nearest integer, ties to even, in the low byte: 1.5 2^23 puts the integer into the last bits of the sum.  The
-// product is rounded first: that brings a tie, which the rounding of inv has moved by less, back to where it is (short
-// numbers are ties often), and gives the plain form's integers.
-__device__ __forceinline__ uint32_t to_int8(float y, float inv) {
-  float p = y * inv;
-  asm("" : "+v"(p));  // (no fma of the two)
+// 127 y / max to the nearest integer, ties to even, in the low byte: 1.5 2^23 puts the integer into the last bits of the sum.  The
+// quotient is rounded to fp32 first, from 48 bits: a tie (short numbers make many) is met as one, where y times the rounded
+// 127 / max alone would lie beside it for a whole row.
+__device__ __forceinline__ uint32_t to_int8(float y, const Step& s) {
+  float p = fmaf(y, s.inv, y * s.rest);
+  asm("" : "+v"(p));  // (no fma with what follows)
   return __float_as_uint(p + 12582912.f);
 }
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -42,7 +43,7 @@ __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, ui
 __device__ __forceinline__ u32x2 pack8(const float (&y)[8], const Step& s) {
   uint32_t u[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) u[j] = to_int8(y[j], s.inv);
+  for (int j = 0; j < 8; ++j) u[j] = to_int8(y[j], s);
   u32x2 r = {pack4(u[0], u[1], u[2], u[3]), pack4(u[4], u[5], u[6], u[7])};
   // (0 times an infinity or a NaN is a NaN, whose bits are no integer)
   if (s.inv == 0.f) r = u32x2{0, 0};

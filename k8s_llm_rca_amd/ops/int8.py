@@ -79,11 +79,11 @@ def _pitch(t: torch.Tensor) -> int:
 
 
 def _quantised(y: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-    """The plain form on the last axis of an fp32 tensor."""
+    """The plain form on the last axis of an fp32 tensor (the quotient in 64 bits, so that ties are ties)."""
     top = y.abs().amax(-1, keepdim=True)
     fine = torch.isfinite(top)
     live = fine & (top >= TINY)
-    q = torch.where(live, torch.round(y * (127.0 / torch.where(live, top, torch.ones_like(top)))), torch.zeros_like(y))
+    q = torch.where(live, torch.round(127 * y.double() / torch.where(live, top, torch.ones_like(top)).double()), 0.0)
     scale = torch.where(live, top / 127.0, torch.where(fine, torch.zeros_like(top), torch.full_like(top, math.nan)))
     return q.to(torch.int8), scale.squeeze(-1)
 

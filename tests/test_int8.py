@@ -119,6 +119,18 @@ def test_rows_that_hold_no_number(device, H):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_ties_go_to_even(device):
+    """Rows of short numbers, every one of which may lie half way between two integers: the integers of the definition, exactly."""
+    top = torch.arange(128, 256, dtype=F64)                   # every bf16 mantissa as the row's maximum
+    x = torch.cat([top[:, None], torch.arange(-128, 129, dtype=F64)[None] * top[:, None] / 256], 1)[:, :256].to(BF)
+    x = torch.cat([x, torch.arange(-127, 129).to(BF).expand(128, -1)], 1).contiguous()
+    x[:, 0] = top.to(BF)
+    x = torch.where(x.double().abs() <= top[:, None], x, torch.zeros((), dtype=BF))
+    q, _ = Q.quantize_rows(x.to(device))
+    assert torch.equal(q.cpu().double(), torch.round(127 * x.double() / top[:, None]))
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_rows_strides_and_outs(device):
     g = gen(3)
     whole = randn(g, 9, 400, dtype=BF, device=device)
