@@ -2,9 +2,12 @@
 //   S = scale ks[j] (q . k[j]),  O = sum_j softmax(S)[j] vs[j] v[j],  key j of row t visible while j < ctx - qlen + t + 1.
 // An int8 is a bf16 exactly, so that both products run on the bf16 matrix instructions with the integers as they are: the
 // key's scale multiplies its score, the value's scale the weight, which is rounded to bf16 with it (the one rounding that is
-// not fp32's: 2^-9 of a weight, as the bf16 cache's attention has it).
+// not fp32's: 2^-8 of a weight, as the bf16 cache's attention has it).  Maxima, sums and O are fp32's.
 //
-// A wave holds 16 rows (token, q head) of one kv head and walks 64 keys at a time.  v_mfma_f32_16x16x32_bf16, S^T = K Q^T:
+// Replies: a wave holds 16 rows (token, q head) of one kv head and walks 64 keys at a time, a run of keys of a list that the host
+// made (long contexts in parts, which meet in a second launch).  What bounds it is the cache's way from memory: 96 replies over 1500
+// to 6000 keys of 8 heads 147 + 5 us, 5.3 TB/s (a large copy moves 5.1); one reply over 5003 keys 7.6 + 4 us, which is
+// latency: loads, softmax and exchange of two chunks a wave, and the second launch.  v_mfma_f32_16x16x32_bf16, S^T = K Q^T:
 // row rho of key tile (u, t) is key 16 (rho >> 2) + 8 u + 4 t + (rho & 3), so that lane group g = lane >> 4 is left with the
 // scores of keys 16 g .. 16 g + 15, whose values of one dim are one 16-byte load, and weights go to the second product
 // without leaving their lane.  Dims of K and Q are taken as 64 c + 16 g + [0, 16) by lane group g: one 16-byte load, two steps.
@@ -65,14 +68,8 @@ __device__ __forceinline__ void load_q(State& st, const AttnArgs& a, long row, i
 
 // Keys [k0, k1) (k0 a multiple of 64) of one sequence; row lane & 15 sees keys below lim, every row those below kmin.
 // A chunk's keys and values make room for the next chunk's as soon as they are used, so that a wave always has 8 to 16 KB on the way.
-template <bool NT>
-__device__ __forceinline__ u32x4 get(const uint8_t* p) {
-  if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
-  return *reinterpret_cast<const u32x4*>(p);
-}
-#ifndef RNT
-#define RNT 1
-#endif
+// They are read non-temporally: a page is read once a step (96 replies over 1500 to 6000 keys 146.6 us, otherwise 151.3).
+__device__ __forceinline__ u32x4 once(const uint8_t* p) { return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)); }
 __device__ __forceinline__ void walk(State& st, const AttnArgs& a, const int* bt, int kvh, int k0, int k1, int kmin, int lim, int lane) {
   const int r = lane & 15, g = lane >> 4, n = (k1 - k0 + 63) >> 6;
   if (n <= 0) return;
@@ -88,14 +85,14 @@ __device__ __forceinline__ void walk(State& st, const AttnArgs& a, const int* bt
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) kf[t][c] = get<RNT>(kb + (at + 4 * t) * D + 64 * c);
+      for (int c = 0; c < 2; ++c) kf[t][c] = once(kb + (at + 4 * t) * D + 64 * c);
       ks[t] = *reinterpret_cast<const f32x4*>(ksb + at + 4 * t);
     }
   };
   auto ask_v = [&](size_t at, int off) {
     const uint8_t* const p = vb + (at - off) * D + off;
 #pragma unroll
-    for (int d = 0; d < 8; ++d) vf[d] = get<RNT>(p + 16 * d * a.BS);
+    for (int d = 0; d < 8; ++d) vf[d] = once(p + 16 * d * a.BS);
   };
   auto ask_vs = [&](size_t at) {
 #pragma unroll
@@ -299,13 +296,16 @@ __global__ void __launch_bounds__(256) reply_merge_kernel(AttnArgs a) {
 // v_mfma_f32_32x32x16_bf16, S^T = K Q^T: row rho of the 32-key half kt is key 32 kt + 16 (reg >> 3) + 8 hi + (reg & 7) with
 // reg = (rho & 3) + 4 (rho >> 3), hi = (rho >> 2) & 1, so that a lane has one row's keys 16 s + 8 hi .. + 7 in registers
 // 8 s .. 8 s + 7: the second operand of O^T += V^T P^T as they are.
-// LDS (three pages of each, so that a turn's first fragments are read in front of its barrier): a key's 256 bytes with 16-byte piece c at c ^ (key & 15), a dim's 128 bytes with piece c at c ^ ((dim >> 1) & 7): no bank
-// conflicts in either direction.
+// LDS (three pages of each, so that a turn's first fragments are read in front of its barrier): a key's 256 bytes with 16-byte
+// piece c at c ^ (key & 15), a dim's 128 bytes with piece c at c ^ ((dim >> 1) & 7): no bank conflicts in either direction.
 // A turn has page i's softmax beside the products of its neighbours, so that the vector and the matrix units work at once: scales,
 // maximum and the weights of the first 32 keys beside V(i - 1), the other weights beside the first half of K(i + 1), whose
 // scores take the registers that the weights have left, the staging beside its second half.  A fixed order of instructions holds it
-// together: left to the compiler, the products come first and the weights behind them (us of the four threads' chunks of
-// up to 2048 tokens over 4000: page after page 585, in turns 576, in this order 507).
+// together: left to the compiler, the products come first and the weights behind them.
+// us of four threads' chunks of up to 2048 tokens over 4000, 32 + 2 x 8 heads: page after page 585, in turns 576, in this order
+// 507, with a turn's first reads in front of its barrier 495 (890 TFLOP/s); a prompt of 8192 567 (969).  What bounds it is the
+// vector unit beside the matrix unit: a turn's 250 vector instructions and 32 exponentials a wave take as long as its 32 products,
+// two waves a SIMD leave some 30 % of both to waits, and tiles of 60 to 94 pages fill 256 units unevenly.
 constexpr int kRows = 256, kPitch = 272;
 constexpr int AHEAD = 3;  // products that a fragment is read in front of its own
 struct ChunkLds {

@@ -87,7 +87,11 @@ __device__ __forceinline__ void put4(const GemmArgs& a, int m, int n, const i32x
 }
 
 // ------------------------------------------------------------ few rows: the weight streams by
-// A workgroup has 16 columns and up to 16 rows; its eight waves cut K into eight runs and meet in LDS.
+// A workgroup has 16 columns and up to 16 rows; its eight waves cut K into eight runs and meet in LDS.  What bounds it is the weight's
+// way: one row of 128256 x 4096 90 us (5.8 TB/s), 28672 x 4096 23.5, 6144 x 4096 8.2 (2 to 3 of them the launch); 16 rows read x
+// as often as w (141 us), so that others take over.  us of one row of 4096 x 4096 / 28672 x 4096 in other forms: eight steps asked
+// for at once 6.7 / 27.4, 16 waves 6.5 / 29.1, waves taking turns over K 6.4 / 30.5, two strips 7.6 / 31.0, non-temporal 5.6 / 24.6,
+// this one 5.8 / 23.2.
 constexpr int kWaves = 8;
 __global__ void __launch_bounds__(64 * kWaves) few_kernel(GemmArgs a) {
   __shared__ i32x4 red[kWaves][64];
@@ -154,7 +158,9 @@ __device__ __forceinline__ void put_part(const GemmArgs& a, int slice, int m, in
 }
 
 // ------------------------------------------------------------ middle sizes: tiles of BM x BN behind a ring of stages
-// Waves 2 x WN; NB stages of 128 bytes of K, NB - 1 of them on their way while one is multiplied; one barrier a stage.
+// Waves 2 x WN; NB stages of 128 bytes of K, NB - 1 of them on their way while one is multiplied; one barrier a stage.  Up to
+// 128 rows the weight's way bounds it (48 rows of 128256 x 4096 108 us, 4.9 TB/s), from then on the stages' way into LDS (some 25
+// bytes a clock and unit): 256 x 4096 x 4096 13 us (660 TOP/s), 1024 x 4096 x 4096 24 us (1430).
 template <int BM, int BN, int NB, int WN>
 __global__ void __launch_bounds__(128 * WN, 2) ring_kernel(GemmArgs a, int n_mt, int n_nt) {
   constexpr int STAGE = (BM + BN) * 128, I = (BM + BN) / (16 * WN);  // DMAs a wave and stage
@@ -240,6 +246,10 @@ __global__ void __launch_bounds__(128 * WN, 2) ring_kernel(GemmArgs a, int n_mt,
 // read once a stage.  Waves 4-7 run one barrier behind waves 0-3, so that on each SIMD one wave multiplies while the other
 // reads.  A half tile is asked for two phases after its place was last read and waited for (four half tiles later still on
 // their way) one phase before it is read.  Rows of w are staged so that a lane's two fragments are eight neighbouring columns.
+// us: 4001 x 28672 x 4096 386 to 394 (2.40 POP/s), 4096 x 4096 x 14336 171 to 177 (2.75), 4096 x 4096 x 4096 56 (2.45); a large bf16
+// product of the library reaches 1.46 PFLOP/s, whose bytes a matrix instruction are the same.  A stage takes 1.5 us, of which the
+// matrix instructions are 1.0: LDS moves as much in the time as it can (192 KB read, 64 KB written a stage); 6 us of each tile
+// are its start and its stores.  What whole rounds of 256 tiles leave has its K cut: 2048 x 10240 x 8192 (320 tiles) 185 -> 155.
 constexpr int HALF = 128 * 128, BUF = 4 * HALF, OX0 = 0, OX1 = HALF, OW0 = 2 * HALF, OW1 = 3 * HALF;
 __global__ void __launch_bounds__(512, 1) big_kernel(GemmArgs a, int n_mt, int n_nt) {
   __shared__ __attribute__((aligned(1024))) uint8_t sm[2 * BUF];
