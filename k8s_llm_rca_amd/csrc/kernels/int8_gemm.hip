@@ -23,6 +23,12 @@ struct GemmArgs {
 };
 __device__ const i32x4 kZeros = {0, 0, 0, 0};
 
+// Whether rows of y take pieces of V values (columns start at multiples of V).
+template <int V>
+__device__ __forceinline__ bool aligned_rows(const GemmArgs& a) {
+  return (a.ldy & (V - 1)) == 0 && ((uintptr_t)a.y & 15) == 0;
+}
+
 // R rows by C pieces of V neighbouring columns: row(i) and col(j) are the row and the first column, at(i, j, e) an integer sum.
 // Scales and bias are asked for together, in front of the first store (a load behind a store waits for both).
 template <int R, int C, int V, typename Row, typename Col, typename At>
@@ -40,7 +46,7 @@ __device__ __forceinline__ void put_block(const GemmArgs& a, Row row, Col col, A
 #pragma unroll
       for (int e = 0; e < V; ++e) b[j][e] = a.bias[min(col(j) + e, a.N - 1)];
   }
-  const bool wide = (a.ldy & (V - 1)) == 0 && ((uintptr_t)a.y & 15) == 0;  // (columns start at multiples of V)
+  const bool wide = aligned_rows<V>(a);
   auto value = [&](int i, int j, int e) { return fmaf((float)at(i, j, e) * f[i], w[j][e], b[j][e]); };
   if (a.f32) {
 #pragma unroll
@@ -84,6 +90,50 @@ __device__ __forceinline__ void put_block(const GemmArgs& a, Row row, Col col, A
 }
 __device__ __forceinline__ void put4(const GemmArgs& a, int m, int n, const i32x4& s) {
   put_block<1, 1, 4>(a, [&](int) { return m; }, [&](int) { return n; }, [&](int, int, int e) { return s[e]; });
+}
+// The same for other rows: R times 16 rows by C times 32 columns of a wave turn in its own LDS (kTurn numbers), 16 by 32 at a time, so that
+// a store has neighbouring lanes at neighbouring columns.  row(i) and col(j) are where they begin; lane (r, g) holds sums
+// at(i, j, e) of row r, e < 8: of columns V (g + 4 (e / V)) + e % V.
+// us of 3655 x 1772 x 2048 and, in fp32, of 484 x 21381 x 432 and 800 x 36639 x 9136: value by value from where they are 47.3, 49.2 and
+// 409, turned with each piece's scales asked for behind the last one's stores 47.0, 33.1 and 337, with all of them in front 35.2, 22.1 and
+// 332 (the next widths that rows start evenly with: 29.6, 22.7 and 322).
+constexpr int kTurnRow = 36, kTurn = 16 * kTurnRow;
+template <int R, int C, int V, typename Row, typename Col, typename At>
+__device__ __forceinline__ void put_turned(const GemmArgs& a, float* lds, int lane, Row row, Col col, At at) {
+  const int r = lane & 15, g = lane >> 4, c = lane & 31, hi = lane >> 5;
+  float f[R], w[C], b[C] = {};
+#pragma unroll
+  for (int i = 0; i < R; ++i) f[i] = a.xs[min(row(i) + r, a.M - 1)];
+#pragma unroll
+  for (int j = 0; j < C; ++j) w[j] = a.ws[min(col(j) + c, a.N - 1)];
+  if (a.bias) {
+#pragma unroll
+    for (int j = 0; j < C; ++j) b[j] = a.bias[min(col(j) + c, a.N - 1)];
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 4)
+        *reinterpret_cast<f32x4*>(lds + r * kTurnRow + V * (g + 4 * (e / V)) + e % V) =
+            f32x4{(float)at(i, j, e) * f[i], (float)at(i, j, e + 1) * f[i], (float)at(i, j, e + 2) * f[i], (float)at(i, j, e + 3) * f[i]};
+      wave_lds_fence();
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = fmaf(lds[(2 * k + hi) * kTurnRow + c], w[j], b[j]);
+      wave_lds_fence();
+      const int m = row(i) + hi, n = col(j) + c;
+      const long o = (long)m * a.ldy + n;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (m + 2 * k >= a.M || n >= a.N) continue;
+        if (a.f32)
+          ((float*)a.y)[o + 2 * k * a.ldy] = v[k];
+        else
+          ((uint16_t*)a.y)[o + 2 * k * a.ldy] = f2bf(v[k]);
+      }
+    }
 }
 
 // ------------------------------------------------------------ few rows: the weight streams by
@@ -236,7 +286,14 @@ __global__ void __launch_bounds__(128 * WN, 2) ring_kernel(GemmArgs a, int n_mt,
       for (int j = 0; j < FN; ++j) put_part(a, slice, row(f), col(j), acc[f][j]);
     return;
   }
-  put_block<FM, FN, 4>(a, row, col, [&](int f, int j, int e) { return acc[f][j][e]; });
+  if (aligned_rows<4>(a)) {
+    put_block<FM, FN, 4>(a, row, col, [&](int f, int j, int e) { return acc[f][j][e]; });
+    return;
+  }
+  bar();  // (every wave is done with the stages)
+  static_assert(FN == 2, "32 columns a wave");
+  put_turned<FM, 1, 4>(a, reinterpret_cast<float*>(sm) + wv * kTurn, lane, [&](int f) { return m0 + wr * (BM / 2) + 16 * f; },
+                       [&](int) { return n0 + wc * (BN / WN); }, [&](int f, int, int e) { return acc[f][e >> 2][e & 3]; });
 }
 
 // ------------------------------------------------------------ large: tiles of 256 x 256, eight phases for two stages
@@ -370,7 +427,13 @@ __global__ void __launch_bounds__(512, 1) big_kernel(GemmArgs a, int n_mt, int n
           *reinterpret_cast<i32x4*>(p + (row(i) - m0) * 256 + col(j) - n0 + 4 * e) = acc[quad(i, j)][i & 3][e];
     return;
   }
-  put_block<8, 2, 8>(a, row, col, [&](int i, int j, int e) { return acc[quad(i, j)][i & 3][e >> 2][e & 3]; });
+  if (aligned_rows<8>(a)) {
+    put_block<8, 2, 8>(a, row, col, [&](int i, int j, int e) { return acc[quad(i, j)][i & 3][e >> 2][e & 3]; });
+    return;
+  }
+  bar();  // (every wave is done with the stages)
+  put_turned<8, 2, 8>(a, reinterpret_cast<float*>(sm) + wv * kTurn, lane, [&](int i) { return m0 + 128 * (i >> 2) + 64 * wr + 16 * (i & 3); },
+                      [&](int j) { return n0 + 128 * j + 32 * wc; }, [&](int i, int j, int e) { return acc[quad(i, j)][i & 3][e >> 2][e & 3]; });
 }
 
 // the runs' sums, scaled: four neighbours a thread
