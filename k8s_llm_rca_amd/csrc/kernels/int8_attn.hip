@@ -42,6 +42,7 @@ struct AttnArgs {
   int n_tiles;
   const int *m_tok0, *m_len, *m_slot0, *m_np;
   int n_merge, slot_rows;
+  int own, parts;  // tokens of a tile that the kernel finds by itself and runs that its keys are cut into; 0: the lists above
 };
 
 struct State {
@@ -324,6 +325,32 @@ __device__ __forceinline__ void each(F&& f) {
 __device__ __forceinline__ void lds_bar() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
+// Tile number t of all sequences' (of `own` tokens each, a sequence's last tokens first: those have the most keys): every lane counts
+// a sequence's.  No tokens where there are fewer tiles, since the launch has as many as T rows of S sequences can have.
+struct Found {
+  int seq, tok0, len;
+};
+__device__ __forceinline__ Found find_tile(const AttnArgs& a, int t) {
+  const int lane = threadIdx.x & 63;
+  for (int s0 = 0; s0 < a.S; s0 += 64) {
+    const int s = min(s0 + lane, a.S - 1), first = a.q_start[s], last = a.q_start[s + 1];
+    const int n = s0 + lane < a.S ? (max(last - first, 0) + a.own - 1) / a.own : 0;
+    int sum = n;  // of this sequence's and those before it
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+      const int below = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += below;
+    }
+    const unsigned long long behind = __ballot(sum > t);
+    if (behind) {
+      const int l = __builtin_ctzll(behind), i = __builtin_amdgcn_readlane(sum, l) - 1 - t, end = __builtin_amdgcn_readlane(last, l);
+      const int tok0 = __builtin_amdgcn_readlane(first, l) + i * a.own;
+      return {s0 + l, tok0, min(a.own, end - tok0)};
+    }
+    t -= __builtin_amdgcn_readlane(sum, 63);
+  }
+  return {0, 0, 0};
+}
 __global__ void __launch_bounds__(512, 1) chunk_kernel(AttnArgs a) {
   __shared__ __attribute__((aligned(1024))) union {
     ChunkLds p;
@@ -332,13 +359,29 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(AttnArgs a) {
   const int kvh = blockIdx.x % a.nkv, tile = blockIdx.x / a.nkv;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, hi = lane >> 5;
-  const int seq = a.tile_seq[tile], tok0 = a.tile_tok0[tile], len = a.tile_len[tile], rows = min(len * a.G, kRows);
+  int seq, tok0, len;
+  if (a.own) {
+    const Found f = find_tile(a, tile / a.parts);
+    if (f.len == 0) return;
+    seq = f.seq, tok0 = f.tok0, len = f.len;
+  } else {
+    seq = a.tile_seq[tile], tok0 = a.tile_tok0[tile], len = a.tile_len[tile];
+  }
+  const int rows = min(len * a.G, kRows);
   const int qs = a.q_start[seq], base = a.ctx[seq] - (a.q_start[seq + 1] - qs) + (tok0 - qs);
   const int* const bt = a.bt + (size_t)seq * a.bt_stride;
   const int grow = 32 * w + r;
   const bool valid = grow < rows;
   const int end = min(base + len, a.bt_stride * a.BS);      // keys of the whole tile
-  const int p0 = a.tile_kv0[tile], np = min(a.tile_kv1[tile], (end + 63) >> 6) - p0;
+  const int all = (end + 63) >> 6;
+  int p0, p1, slot = -1;
+  if (a.own) {
+    p0 = max(all, 0) * (tile % a.parts) / a.parts, p1 = max(all, 0) * (tile % a.parts + 1) / a.parts;
+    if (a.parts > 1) slot = tile;
+  } else {
+    p0 = a.tile_kv0[tile], p1 = min(a.tile_kv1[tile], all), slot = a.tile_slot[tile];
+  }
+  const int np = p1 - p0;
   // this lane's row sees keys below `limit`, every row of the wave those below `lo`
   const int limit = min(valid ? base + grow / a.G + 1 : 0, end), lo = 32 * w + 31 < rows ? base + 32 * w / a.G + 1 : 0;
 
@@ -568,7 +611,6 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(AttnArgs a) {
       if constexpr (j + AHEAD < 16) fr[(j + AHEAD) & 3] = fragment(ic<j + AHEAD>{}, s2, 0);
     });
   }
-  const int slot = a.tile_slot[tile];
   l += __shfl_xor(l, 32, 64);
   if (slot >= 0) {
     if (!valid) return;
@@ -610,12 +652,19 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(AttnArgs a) {
   }
 }
 
-// rows of split tiles: grid (n_merge * nkv, rows)
+// rows of split tiles: grid (split tiles * nkv, rows)
 __global__ void __launch_bounds__(64) chunk_merge_kernel(AttnArgs a) {
   const int kvh = blockIdx.x % a.nkv, mi = blockIdx.x / a.nkv, row = blockIdx.y;
-  if (row >= a.m_len[mi] * a.G) return;
-  join_parts<2>(a.part_o, a.part_ml, ((size_t)a.m_slot0[mi] * a.nkv + kvh) * a.slot_rows + row, (size_t)a.nkv * a.slot_rows, a.m_np[mi],
-                a.out + (long)(a.m_tok0[mi] + row / a.G) * a.ldo + (kvh * a.G + row % a.G) * D);
+  int tok0, len, slot0, np;
+  if (a.own) {
+    const Found f = find_tile(a, mi);
+    tok0 = f.tok0, len = f.len, slot0 = mi * a.parts, np = a.parts;
+  } else {
+    tok0 = a.m_tok0[mi], len = a.m_len[mi], slot0 = a.m_slot0[mi], np = a.m_np[mi];
+  }
+  if (row >= len * a.G) return;
+  join_parts<2>(a.part_o, a.part_ml, ((size_t)slot0 * a.nkv + kvh) * a.slot_rows + row, (size_t)a.nkv * a.slot_rows, np,
+                a.out + (long)(tok0 + row / a.G) * a.ldo + (kvh * a.G + row % a.G) * D);
 }
 
 }  // namespace q8
@@ -640,27 +689,30 @@ K8S_API int k8s_int8_attn_reply(const void* q, long ldq, const void* k, const vo
   return (int)hipGetLastError();
 }
 
-// tiles of up to `rows` (token, q head) rows; split tiles leave parts of slot_rows rows a slot and kv head
+// Tiles of up to `rows` (token, q head) rows; split tiles leave parts of slot_rows rows a slot and kv head.  With own > 0 the lists are not
+// read: n_tiles is the most tiles of `own` tokens that the rows can make, and each one's keys are cut into `parts` runs.
 K8S_API int k8s_int8_attn_chunk(const void* q, long ldq, const void* k, const void* v, const float* ks, const float* vs, int NB, const int* bt,
-                                int bt_stride, const int* ctx, const int* q_start, int nq, int nkv, int BS, float scale, void* out, long ldo,
+                                int bt_stride, const int* ctx, const int* q_start, int S, int nq, int nkv, int BS, float scale, void* out, long ldo,
                                 const int* tile_seq, const int* tile_tok0, const int* tile_len, const int* tile_kv0, const int* tile_kv1,
                                 const int* tile_slot, int n_tiles, int rows, const int* m_tok0, const int* m_len, const int* m_slot0,
-                                const int* m_np, int n_merge, float* part_o, float* part_ml, int slot_rows, void* stream) {
+                                const int* m_np, int n_merge, float* part_o, float* part_ml, int slot_rows, int own, int parts, void* stream) {
   using namespace k8s::q8;
   if (n_tiles <= 0) return 0;
   if (nkv <= 0 || nq % nkv || BS <= 0 || (BS & 63) || NB <= 0 || rows <= 0 || rows > kRows || rows > slot_rows) return (int)hipErrorInvalidValue;
-  if (n_merge > 0 && (!part_o || !part_ml)) return (int)hipErrorInvalidValue;
+  if (own < 0 || (own > 0 && (parts <= 0 || S <= 0 || (long)own * (nq / nkv) > rows))) return (int)hipErrorInvalidValue;
+  const int runs = own > 0 ? parts : 1, merged = own > 0 ? (parts > 1 ? n_tiles : 0) : n_merge;
+  if (merged > 0 && (!part_o || !part_ml)) return (int)hipErrorInvalidValue;
   AttnArgs a{};
   a.q = (const uint16_t*)q, a.ldq = ldq, a.k = (const uint8_t*)k, a.v = (const uint8_t*)v, a.ks = ks, a.vs = vs, a.bt = bt;
-  a.bt_stride = bt_stride, a.NB = NB, a.ctx = ctx, a.q_start = q_start, a.nq = nq, a.nkv = nkv, a.G = nq / nkv, a.BS = BS;
-  a.scale_log2 = scale * kLog2e, a.out = (uint16_t*)out, a.ldo = ldo, a.part_o = part_o, a.part_ml = part_ml;
+  a.bt_stride = bt_stride, a.NB = NB, a.ctx = ctx, a.q_start = q_start, a.S = S, a.nq = nq, a.nkv = nkv, a.G = nq / nkv, a.BS = BS;
+  a.scale_log2 = scale * kLog2e, a.out = (uint16_t*)out, a.ldo = ldo, a.part_o = part_o, a.part_ml = part_ml, a.own = own, a.parts = runs;
   a.tile_seq = tile_seq, a.tile_tok0 = tile_tok0, a.tile_len = tile_len, a.tile_kv0 = tile_kv0, a.tile_kv1 = tile_kv1, a.tile_slot = tile_slot;
   a.n_tiles = n_tiles, a.m_tok0 = m_tok0, a.m_len = m_len, a.m_slot0 = m_slot0, a.m_np = m_np;
   a.n_merge = n_merge, a.slot_rows = slot_rows;
   hipStream_t st = (hipStream_t)stream;
-  const long blocks = (long)n_tiles * nkv;
+  const long blocks = (long)n_tiles * runs * nkv;
   if (blocks > 0x7fffffffL) return (int)hipErrorInvalidValue;
   hipLaunchKernelGGL(chunk_kernel, dim3((unsigned)blocks), dim3(512), 0, st, a);
-  if (n_merge > 0) hipLaunchKernelGGL(chunk_merge_kernel, dim3(n_merge * nkv, rows), dim3(64), 0, st, a);
+  if (merged > 0) hipLaunchKernelGGL(chunk_merge_kernel, dim3(merged * nkv, rows), dim3(64), 0, st, a);
   return (int)hipGetLastError();
 }

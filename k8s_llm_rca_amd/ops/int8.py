@@ -349,13 +349,24 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
         raise ValueError(f"{G} query heads a key head: a tile takes {A.PF8_ROWS}")
     if meta.tile_seq is None or meta.tile_kv1 is None:
         raise ValueError("the step has no plan: attach_plan")
-    part_o, part_ml = meta.pf_o, meta.pf_ml
-    if meta.n_merge and part_o is None:  # (a split tile's parts are tiles of the plan: no more than those, without a look at the device)
-        part_o = scratch(meta.n_tiles * nkv * A.PF8_ROWS * D, torch.float32, q.device)
-        part_ml = scratch(meta.n_tiles * nkv * A.PF8_ROWS * 2, torch.float32, q.device)
-    _call("k8s_int8_attn_chunk", dev, *common, nq, nkv, BS, scale, out.data_ptr(), ldo, ptr(meta.tile_seq), ptr(meta.tile_tok0),
-          ptr(meta.tile_len), ptr(meta.tile_kv0), ptr(meta.tile_kv1), ptr(meta.tile_slot), meta.n_tiles, rows, ptr(meta.m_tok0),
-          ptr(meta.m_len), ptr(meta.m_slot0), ptr(meta.m_np), meta.n_merge, ptr(part_o), ptr(part_ml), A.PF8_ROWS)
+    part_o, part_ml, tiles, merged, own, runs = meta.pf_o, meta.pf_ml, meta.n_tiles, meta.n_merge, 0, 1
+    if rows <= 64 and rows < A.PF8_ROWS // G * G:
+        # Where heads or pages do not fit the bf16 cache's kernels the plan has tiles of 64 rows over whole key ranges.  A workgroup
+        # here takes 256 rows and finds them by itself.  Few of them cut their keys until there are as many as compute units, of
+        # five pages each at least; from half as many on they make two rounds, which even out short and long tiles.  us by the plan's
+        # tiles and by these, 10 + 2 x 2 heads: six threads' six tokens over 8064 keys 260 and 27, a prompt of 4096 225 and 97, two
+        # of 513 27 and 26; 12 + 2 x 4: two chunks of 2000 over 2000 273 and 114, six prompts of 234 17.7 and 18.4.
+        own = min(A.PF8_ROWS // G, T)
+        tiles, merged, rows = T // own + S, 0, own * G
+        blocks, pages = tiles * nkv, bt.shape[1] * BS // 64
+        runs = max(1, min(256 // blocks, pages // 5) if blocks <= 128 else min(512 // blocks, pages // 16))
+        part_o = None
+    if part_o is None and (merged or runs > 1):  # (a split tile's parts are tiles of the plan: no more than those, without a look at the device)
+        part_o = scratch(tiles * runs * nkv * A.PF8_ROWS * D, torch.float32, q.device)
+        part_ml = scratch(tiles * runs * nkv * A.PF8_ROWS * 2, torch.float32, q.device)
+    _call("k8s_int8_attn_chunk", dev, *common, S, nq, nkv, BS, scale, out.data_ptr(), ldo, ptr(meta.tile_seq), ptr(meta.tile_tok0),
+          ptr(meta.tile_len), ptr(meta.tile_kv0), ptr(meta.tile_kv1), ptr(meta.tile_slot), tiles, rows, ptr(meta.m_tok0),
+          ptr(meta.m_len), ptr(meta.m_slot0), ptr(meta.m_np), merged, ptr(part_o), ptr(part_ml), A.PF8_ROWS, own, runs)
     return out
 
 

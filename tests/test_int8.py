@@ -523,6 +523,46 @@ def test_chunk(device, lens, nq, nkv, BS):
     check_attention(out, q, cache, meta, starts, ctx, nq, nkv, 0.09)
 
 
+# heads and pages whose tiles the kernel finds by itself: keys cut and whole, sequences without rows, with fewer keys than rows and in
+# more groups of 64 than one, a table wider than any context
+OWN = [([(6, 2000), (0, 500), (3, 3)], 10, 2, 64, 0), ([(1, 1)] + [(0, 70)] * 70 + [(2, 130), (60, 60)], 12, 4, 64, 0), ([(400, 900)], 10, 10, 128, 0),
+       ([(5, 40), (52, 52), (51, 300)], 10, 2, 64, 60), ([(7, 900)] * 3, 6, 2, 256, 0), ([(3, 700)], 100, 1, 64, 0), ([(20, 9), (3, 400)], 10, 2, 64, 0),
+       ([(2500, 3000)], 10, 2, 64, 0)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,nq,nkv,BS,more", OWN)
+def test_chunk_of_uneven_heads(lens, nq, nkv, BS, more):
+    q, cache, meta, starts, ctx = attn_case("cuda", lens, nq, nkv, BS)
+    if more:
+        meta.block_tables = torch.cat([meta.block_tables, torch.zeros(len(lens), more, dtype=torch.int32, device="cuda")], 1).contiguous()
+    A.attach_plan(meta, A.plan_prefill(starts, nq // nkv, BS), "cuda")
+    out = torch.full((starts[-1] + 2, nq * D), 7.0, dtype=BF, device="cuda")     # (two padding rows)
+    q = torch.cat([q, q[:2]])
+    Q.paged_attention_int8(q, cache, meta, nq, nkv, 0.09, out=out)
+    check_attention(out, q, cache, meta, starts, ctx, nq, nkv, 0.09)
+    assert bool((out[starts[-1]:] == 7).all())
+
+
+@pytest.mark.gpu
+def test_a_captured_chunk_of_uneven_heads_follows_its_lengths():
+    """What a step's sequences have is read when it is replayed, here in 77 rows that one, three or no sequences share."""
+    q, cache, meta, starts, ctx = attn_case("cuda", [(7, 600), (60, 700), (10, 400)], 10, 2)
+    A.attach_plan(meta, A.plan_prefill(starts, 5, 64), "cuda")
+    Q.paged_attention_int8(q, cache, meta, 10, 2, 0.09)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = Q.paged_attention_int8(q, cache, meta, 10, 2, 0.09)
+    for starts, ctx in (([0, 7, 67, 77], [600, 700, 400]), ([0, 0, 77, 77], [5, 90, 1]), ([0, 30, 31, 40], [30, 700, 9]), ([0, 0, 0, 0], [1, 1, 1])):
+        meta.q_start.copy_(torch.tensor(starts, dtype=torch.int32))
+        meta.ctx_lens.copy_(torch.tensor(ctx, dtype=torch.int32))
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        check_attention(out, q, cache, meta, starts, ctx, 10, 2, 0.09)
+        assert bool((out[starts[-1]:] == 7).all())
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_rows_in_front_of_their_context_are_zero(device):
     """More new rows than the context has: the first ones see no key."""
