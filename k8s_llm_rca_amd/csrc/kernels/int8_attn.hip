@@ -476,140 +476,155 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(AttnArgs a) {
     ask_v();
     for (int i = tid; i < D * 8; i += 512) *reinterpret_cast<u32x4*>(sm.p.v[2] + 16 * i) = u32x4{0, 0, 0, 0};  // (page -1's weights are zeros)
     lds_bar();
-    each<16>([&](auto J) { product(ic<decltype(J)::value + 16>{}, fragment(ic<decltype(J)::value + 16>{}, 0, 0)); });
-    auto four = [](const float* f, int g) { return *reinterpret_cast<const f32x4*>(f + 16 * (g >> 1) + 4 * (g & 1)); };  // of a lane's scores 4g ..
-    auto hide = [&](int i) {  // keys that the row does not see
-      const int k0 = 64 * (p0 + i) + 8 * hi;
-#pragma unroll
-      for (int e = 0; e < 32; ++e)
-        if (k0 + 16 * (e >> 3) + (e & 7) >= limit) sc[e >> 4][e & 15] = -INFINITY;
-    };
-    auto largest = [&] {
-      float c0 = -INFINITY, c1 = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        c0 = fmaxf(c0, sc[0][e]);
-        c1 = fmaxf(c1, sc[1][e]);
-      }
-      return fmaxf(c0, c1);
-    };
-    auto of_row = [](float top) {  // the two halves of a row
-      const auto pr = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-      return fmaxf(__uint_as_float(pr[0]), __uint_as_float(pr[1]));
-    };
-    {
-      // where the row's weights begin: the largest score of the first page (a row without a key there has none at all)
-      const f32x16 raw[2] = {sc[0], sc[1]};
-#pragma unroll
-      for (int g = 0; g < 8; ++g) {
-        const f32x4 f = four(sm.p.s[0][0] + 8 * hi, g);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sc[g >> 2][4 * (g & 3) + e] *= f[e];
-      }
-      hide(0);
-      const float top = of_row(largest());
-      m = top == -INFINITY ? 0.f : top;
-      sc[0] = raw[0], sc[1] = raw[1];
-    }
-    bf16x8 fr[4];
-    f32x4 fs[4];
-    // scales of four keys: of keys 4q .. of a lane, wanted by step q (q < 8), of values 4(q - 8) .., wanted by step 2 q - 8; read
-    // three steps in front
-    auto scale = [&](auto Q, int i) {
-      constexpr int q = decltype(Q)::value;
-      fs[q & 3] = four(sm.p.s[i & 3][q >> 3] + 8 * hi, q & 7);
-    };
-    each<3>([&](auto J) {
-      scale(J, 0);
-      fr[J] = fragment(J, 2, 1);
-    });
     int s0 = 0, s1 = 1, s2 = 2;  // i, i + 1 and i + 2 by three
-    for (int i = 0; i < np; ++i) {
-      lds_bar();  // K(i + 2) and V(i) are there, every wave is done with K(i) and V(i - 2)
-      uint32_t pn[16];
-      float c[2] = {-INFINITY, -INFINITY}, sum[4] = {0.f, 0.f, 0.f, 0.f}, up = 0.f;
-      each<32>([&](auto Jc) {
-        constexpr int j = decltype(Jc)::value;
-        if constexpr (j + AHEAD < 32)
-          fr[(j + AHEAD) & 3] = fragment(ic<j + AHEAD>{}, s2, s1);
-        else
-          fr[(j + AHEAD) & 3] = fragment(ic<j + AHEAD - 32>{}, s0, s2);  // the next turn's
-        if constexpr (j < 5)
-          scale(ic<j + 3>{}, i);
-        else if constexpr (j < 20 && (j & 1))
-          scale(ic<(j + 11) / 2>{}, i);
-        else if constexpr (j >= 29)
-          scale(ic<j - 29>{}, i + 1);
-        product(Jc, fr[j & 3]);
-        if constexpr (j < 8) {  // four scores of the lane, above what the row's weights stand on
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = fmaf(sc[j >> 2][4 * (j & 3) + e], fs[j & 3][e], -m);
-            asm volatile("" : "+v"(x));  // (not made again from the sum and the scale, which would stay in registers for it)
-            sc[j >> 2][4 * (j & 3) + e] = x;
-            c[e & 1] = fmaxf(c[e & 1], x);
-          }
-        } else if constexpr (j < 24) {  // two weights
-          if constexpr (j == 8) {
-            float top = fmaxf(c[0], c[1]);
-            if (64 * (p0 + i) + 64 > lo) {
-              hide(i);
-              top = largest();
-            }
-            top = of_row(top);
-            // where a row grows by more than 8, its weights stand on its new maximum from here on: weights up to 2^8
-            if (__ballot(top > 8.f)) {
-              up = top > 8.f ? top : 0.f;
-              m += up;
-#pragma unroll
-              for (int e = 0; e < 32; ++e) sc[e >> 4][e & 15] -= up;
-            }
-          }
-          constexpr int t = j - 8, kt = t >> 3, e = 2 * (t & 7);
-          const float x0 = __builtin_amdgcn_exp2f(sc[kt][e]), x1 = __builtin_amdgcn_exp2f(sc[kt][e + 1]);
-          sum[2 * (t & 1)] += x0;
-          sum[2 * (t & 1) + 1] += x1;
-          typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-          uint32_t two = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)(x0 * fs[(t >> 1) & 3][e & 3]), (__bf16)(x1 * fs[(t >> 1) & 3][(e & 3) + 1])});
-          // (wanted in the next turn only: computed here all the same, beside the products)
-          asm volatile("" : "+v"(two), "+v"(sum[2 * (t & 1)]), "+v"(sum[2 * (t & 1) + 1]));
-          pn[t] = two;
-        } else if constexpr (j == 24) {
-          keep_k(i + 3, s0);
-        } else if constexpr (j == 27) {
-          ask_k(i + 4);
-        } else if constexpr (j == 28) {
-          keep_v(s1);
-        } else if constexpr (j == 30) {
-          ask_v();
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      });
-      if (((i + 5) & 63) == 0 && i + 5 < np) ids = ids_from(i + 5);
-      if (__ballot(up != 0.f)) {
-        const float alpha = __builtin_amdgcn_exp2f(-up);
-        l *= alpha;
-#pragma unroll
-        for (int d = 0; d < 4; ++d)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
+    // A wave without rows stages its share and nothing else: the others have its time.  (us of eight threads' 12 tokens over 7332 keys,
+    // 16 + 2 x 16 heads, 133 -> 99; five threads' 24 over 7398, 32 + 2 x 8, 46 -> 37.)
+    if (32 * w >= rows) {
+      for (int i = 0; i < np; ++i) {
+        lds_bar();
+        keep_k(i + 3, s0);
+        ask_k(i + 4);
+        keep_v(s1);
+        ask_v();
+        if (((i + 5) & 63) == 0 && i + 5 < np) ids = ids_from(i + 5);
+        const int s3 = s0;
+        s0 = s1, s1 = s2, s2 = s3;
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const uint32_t* const t = pn + 8 * kt + 4 * s;
-          pf[kt][s] = __builtin_bit_cast(bf16x8, u32x4{t[0], t[1], t[2], t[3]});
+    } else {
+      each<16>([&](auto J) { product(ic<decltype(J)::value + 16>{}, fragment(ic<decltype(J)::value + 16>{}, 0, 0)); });
+      auto four = [](const float* f, int g) { return *reinterpret_cast<const f32x4*>(f + 16 * (g >> 1) + 4 * (g & 1)); };  // of a lane's scores 4g ..
+      auto hide = [&](int i) {  // keys that the row does not see
+        const int k0 = 64 * (p0 + i) + 8 * hi;
+  #pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (k0 + 16 * (e >> 3) + (e & 7) >= limit) sc[e >> 4][e & 15] = -INFINITY;
+      };
+      auto largest = [&] {
+        float c0 = -INFINITY, c1 = -INFINITY;
+  #pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          c0 = fmaxf(c0, sc[0][e]);
+          c1 = fmaxf(c1, sc[1][e]);
         }
-      const int s3 = s0;
-      s0 = s1, s1 = s2, s2 = s3;
+        return fmaxf(c0, c1);
+      };
+      auto of_row = [](float top) {  // the two halves of a row
+        const auto pr = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+        return fmaxf(__uint_as_float(pr[0]), __uint_as_float(pr[1]));
+      };
+      {
+        // where the row's weights begin: the largest score of the first page (a row without a key there has none at all)
+        const f32x16 raw[2] = {sc[0], sc[1]};
+  #pragma unroll
+        for (int g = 0; g < 8; ++g) {
+          const f32x4 f = four(sm.p.s[0][0] + 8 * hi, g);
+  #pragma unroll
+          for (int e = 0; e < 4; ++e) sc[g >> 2][4 * (g & 3) + e] *= f[e];
+        }
+        hide(0);
+        const float top = of_row(largest());
+        m = top == -INFINITY ? 0.f : top;
+        sc[0] = raw[0], sc[1] = raw[1];
+      }
+      bf16x8 fr[4];
+      f32x4 fs[4];
+      // scales of four keys: of keys 4q .. of a lane, wanted by step q (q < 8), of values 4(q - 8) .., wanted by step 2 q - 8; read
+      // three steps in front
+      auto scale = [&](auto Q, int i) {
+        constexpr int q = decltype(Q)::value;
+        fs[q & 3] = four(sm.p.s[i & 3][q >> 3] + 8 * hi, q & 7);
+      };
+      each<3>([&](auto J) {
+        scale(J, 0);
+        fr[J] = fragment(J, 2, 1);
+      });
+      for (int i = 0; i < np; ++i) {
+        lds_bar();  // K(i + 2) and V(i) are there, every wave is done with K(i) and V(i - 2)
+        uint32_t pn[16];
+        float c[2] = {-INFINITY, -INFINITY}, sum[4] = {0.f, 0.f, 0.f, 0.f}, up = 0.f;
+        each<32>([&](auto Jc) {
+          constexpr int j = decltype(Jc)::value;
+          if constexpr (j + AHEAD < 32)
+            fr[(j + AHEAD) & 3] = fragment(ic<j + AHEAD>{}, s2, s1);
+          else
+            fr[(j + AHEAD) & 3] = fragment(ic<j + AHEAD - 32>{}, s0, s2);  // the next turn's
+          if constexpr (j < 5)
+            scale(ic<j + 3>{}, i);
+          else if constexpr (j < 20 && (j & 1))
+            scale(ic<(j + 11) / 2>{}, i);
+          else if constexpr (j >= 29)
+            scale(ic<j - 29>{}, i + 1);
+          product(Jc, fr[j & 3]);
+          if constexpr (j < 8) {  // four scores of the lane, above what the row's weights stand on
+  #pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float x = fmaf(sc[j >> 2][4 * (j & 3) + e], fs[j & 3][e], -m);
+              asm volatile("" : "+v"(x));  // (not made again from the sum and the scale, which would stay in registers for it)
+              sc[j >> 2][4 * (j & 3) + e] = x;
+              c[e & 1] = fmaxf(c[e & 1], x);
+            }
+          } else if constexpr (j < 24) {  // two weights
+            if constexpr (j == 8) {
+              float top = fmaxf(c[0], c[1]);
+              if (64 * (p0 + i) + 64 > lo) {
+                hide(i);
+                top = largest();
+              }
+              top = of_row(top);
+              // where a row grows by more than 8, its weights stand on its new maximum from here on: weights up to 2^8
+              if (__ballot(top > 8.f)) {
+                up = top > 8.f ? top : 0.f;
+                m += up;
+  #pragma unroll
+                for (int e = 0; e < 32; ++e) sc[e >> 4][e & 15] -= up;
+              }
+            }
+            constexpr int t = j - 8, kt = t >> 3, e = 2 * (t & 7);
+            const float x0 = __builtin_amdgcn_exp2f(sc[kt][e]), x1 = __builtin_amdgcn_exp2f(sc[kt][e + 1]);
+            sum[2 * (t & 1)] += x0;
+            sum[2 * (t & 1) + 1] += x1;
+            typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+            uint32_t two = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)(x0 * fs[(t >> 1) & 3][e & 3]), (__bf16)(x1 * fs[(t >> 1) & 3][(e & 3) + 1])});
+            // (wanted in the next turn only: computed here all the same, beside the products)
+            asm volatile("" : "+v"(two), "+v"(sum[2 * (t & 1)]), "+v"(sum[2 * (t & 1) + 1]));
+            pn[t] = two;
+          } else if constexpr (j == 24) {
+            keep_k(i + 3, s0);
+          } else if constexpr (j == 27) {
+            ask_k(i + 4);
+          } else if constexpr (j == 28) {
+            keep_v(s1);
+          } else if constexpr (j == 30) {
+            ask_v();
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        });
+        if (((i + 5) & 63) == 0 && i + 5 < np) ids = ids_from(i + 5);
+        if (__ballot(up != 0.f)) {
+          const float alpha = __builtin_amdgcn_exp2f(-up);
+          l *= alpha;
+  #pragma unroll
+          for (int d = 0; d < 4; ++d)
+  #pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  #pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+  #pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const uint32_t* const t = pn + 8 * kt + 4 * s;
+            pf[kt][s] = __builtin_bit_cast(bf16x8, u32x4{t[0], t[1], t[2], t[3]});
+          }
+        const int s3 = s0;
+        s0 = s1, s1 = s2, s2 = s3;
+      }
+      each<16>([&](auto J) {  // (V(np - 1) is at s2)
+        constexpr int j = decltype(J)::value;
+        product(J, fr[j & 3]);
+        if constexpr (j + AHEAD < 16) fr[(j + AHEAD) & 3] = fragment(ic<j + AHEAD>{}, s2, 0);
+      });
     }
-    each<16>([&](auto J) {  // (V(np - 1) is at s2)
-      constexpr int j = decltype(J)::value;
-      product(J, fr[j & 3]);
-      if constexpr (j + AHEAD < 16) fr[(j + AHEAD) & 3] = fragment(ic<j + AHEAD>{}, s2, 0);
-    });
   }
   l += __shfl_xor(l, 32, 64);
   if (slot >= 0) {

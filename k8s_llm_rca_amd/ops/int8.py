@@ -350,8 +350,8 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
     if meta.tile_seq is None or meta.tile_kv1 is None:
         raise ValueError("the step has no plan: attach_plan")
     part_o, part_ml, tiles, merged, own, runs = meta.pf_o, meta.pf_ml, meta.n_tiles, meta.n_merge, 0, 1
-    if rows <= 64 and rows < A.PF8_ROWS // G * G:
-        # Where heads or pages do not fit the bf16 cache's kernels the plan has tiles of 64 rows over whole key ranges.  A workgroup
+    if A.PF_ROWS % G or BS != 64:
+        # Where heads or pages do not fit the bf16 cache's kernels the plan has tiles of about 64 rows over whole key ranges.  A workgroup
         # here takes 256 rows and finds them by itself.  Few of them cut their keys until there are as many as compute units, of
         # five pages each at least; from half as many on they make two rounds, which even out short and long tiles.  us by the plan's
         # tiles and by these, 10 + 2 x 2 heads: six threads' six tokens over 8064 keys 260 and 27, a prompt of 4096 225 and 97, two
