@@ -323,6 +323,8 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
         return _attention_plain(q, cache, meta, nq, nkv, scale, out)
     if bt.dtype != torch.int32 or bt.dim() != 2 or bt.shape[0] < S or bt.stride(1) != 1:
         raise ValueError("block_tables must be int32 [S, pages]")
+    if S > 1 and bt.stride(0) < bt.shape[1]:
+        raise ValueError("the rows of block_tables overlap")
     if ctx.dtype != torch.int32 or starts.dtype != torch.int32 or ctx.numel() < S or starts.numel() < S + 1:
         raise ValueError("ctx_lens must be int32 [S] and q_start int32 [S + 1]")
     ldq = _pitch(q)
@@ -338,6 +340,7 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
             raise ValueError(f"{G} query heads a key head: a reply step takes 16")
         if meta.items is None or meta.items.dtype != torch.int32:
             raise ValueError("the step has no plan: attach_decode_plan")
+        _planned(dev, meta.items, meta.d_n_items, meta.part_o, meta.part_ml)
         if meta.n_parts > 1 and meta.part_o is None:
             raise ValueError("a plan of several parts needs part_o and part_ml")
         grid = max(1, meta.grid_waves or min(A.DECODE_WAVE_SLOTS, meta.n_items * nkv))
@@ -349,6 +352,8 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
         raise ValueError(f"{G} query heads a key head: a tile takes {A.PF8_ROWS}")
     if meta.tile_seq is None or meta.tile_kv1 is None:
         raise ValueError("the step has no plan: attach_plan")
+    _planned(dev, meta.tile_seq, meta.tile_tok0, meta.tile_len, meta.tile_kv0, meta.tile_kv1, meta.tile_slot, meta.m_tok0, meta.m_len, meta.m_slot0,
+             meta.m_np, meta.pf_o, meta.pf_ml)
     part_o, part_ml, tiles, merged, own, runs = meta.pf_o, meta.pf_ml, meta.n_tiles, meta.n_merge, 0, 1
     if A.PF_ROWS % G or BS != 64:
         # Where heads or pages do not fit the bf16 cache's kernels the plan has tiles of about 64 rows over whole key ranges.  A workgroup
@@ -368,6 +373,12 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
           ptr(meta.tile_len), ptr(meta.tile_kv0), ptr(meta.tile_kv1), ptr(meta.tile_slot), tiles, rows, ptr(meta.m_tok0),
           ptr(meta.m_len), ptr(meta.m_slot0), ptr(meta.m_np), merged, ptr(part_o), ptr(part_ml), A.PF8_ROWS, own, runs)
     return out
+
+
+def _planned(dev: int, *arrays) -> None:
+    for t in arrays:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"a plan on {t.device} for device {dev}")
 
 
 def _attention_plain(q, cache: Int8KV, meta: A.AttnMeta, nq, nkv, scale, out):

@@ -713,6 +713,20 @@ def test_refusals_on_the_device():
         Q.linear_int8(x[:, :48], s, torch.zeros(4, 65, dtype=torch.int8, device="cuda")[:, 1:49], s)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,nq", [([(1, 70), (1, 3)], 4), ([(2, 70), (3, 3)], 4), ([(2, 70), (3, 3)], 6)])
+def test_refusals_of_plans_and_tables(lens, nq):
+    q, cache, meta, starts, ctx = attn_case("cuda", lens, nq, 2)
+    planned(meta, starts, ctx, nq, 2, 64, device="cpu")        # a plan that the device cannot read
+    with pytest.raises(ValueError):
+        Q.paged_attention_int8(q, cache, meta, nq, 2, 1.0)
+    planned(meta, starts, ctx, nq, 2, 64)
+    Q.paged_attention_int8(q, cache, meta, nq, 2, 1.0)
+    meta.block_tables = meta.block_tables[:1].expand(2, -1)    # rows of no length of their own
+    with pytest.raises(ValueError):
+        Q.paged_attention_int8(q, cache, meta, nq, 2, 1.0)
+
+
 # ------------------------------------------------------------------ together
 class Layer:
     """A decoder layer in 8 bits, as the module's docstring has it."""
