@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(128 * WN, 2) ring_kernel(GemmArgs a, int n_mt,
     return;
   }
   bar();  // (every wave is done with the stages)
-  static_assert(FN == 2, "32 columns a wave");
+  static_assert(FN == 2 && (BM + BN) % (16 * WN) == 0, "32 columns and whole DMAs a wave");
   put_turned<FM, 1, 4>(a, reinterpret_cast<float*>(sm) + wv * kTurn, lane, [&](int f) { return m0 + wr * (BM / 2) + 16 * f; },
                        [&](int) { return n0 + wc * (BN / WN); }, [&](int f, int, int e) { return acc[f][e >> 2][e & 3]; });
 }
@@ -463,19 +463,21 @@ __global__ void __launch_bounds__(256) join_big_kernel(GemmArgs a, int n_mt, int
 
 // ------------------------------------------------------------ the choice
 // Rows and columns of a tile by kind.
-constexpr int kEdge[7][2] = {{16, 16}, {32, 64}, {64, 64}, {64, 128}, {128, 64}, {128, 128}, {256, 256}};
+constexpr int kEdge[8][2] = {{16, 16}, {32, 64}, {64, 64}, {64, 128}, {128, 64}, {128, 128}, {256, 256}, {128, 256}};
 
 // Estimated us of a product.  Its tiles take rounds over the 256 compute units, a round `per` stages of 128 bytes of K and a fixed part;
-// the middle tiles lie two on a unit, where a stage takes longer.  Beside that stands the weight's way from memory: the third
+// the smaller of the middle tiles lie two on a unit, where a stage takes longer.  Beside that stands the weight's way from memory: the third
 // root of the cubes' sum, roughly, since the one hides in the other until they are alike.  Few rows: the weight's way with the
 // rows' reads beside it, against the latency of each wave's turns over K (four steps of 64 bytes a turn), and what a workgroup
 // costs beside its loads, which shows where K is short.  The constants are a fit to times of every kind and cut at 480 sizes: 1 to
 // 4096 rows by 16 weights of 512 x 512 to 128256 x 4096 (K from 512 to 28672), the weights from memory.  The choice is 1.3 % from
 // the best one on average; furthest off are 13 and 16 rows of 5120 x 5120, 14.6 and 16.0 us for 10.9.
+// Tiles of 128 x 256 came later (96 sizes, 72 to 1000 rows: 0.4 % from the best one, without them 4.1; 512 rows of 14336 x 4096 46.6 -> 38.4 us,
+// 128 of 40000 x 4096 54.9 -> 46.6, 256 of 28672 x 4096 48.4 -> 43.4, 100 of 128256 x 4096 134 -> 126).
 inline double cost(int M, int N, int K, int kind, int splits) {
   constexpr double kStart = 2.62, kByte = 0.150e-6, kJoin = 2.46, kJoinByte = 0.328e-6;
-  // us a stage alone on a unit, by twos (of the two largest: with few units busy), a round's fixed part
-  constexpr double c[7][3] = {{}, {.260, .434, 1.54}, {.361, .525, 1.44}, {.453, .809, 1.60}, {.592, .800, 2.00}, {.643, .542, 2.61}, {1.44, .995, 5.61}};
+  // us a stage alone on a unit, by twos (of the three largest, a round full and nearly empty), a round's fixed part
+  constexpr double c[8][3] = {{}, {.260, .434, 1.54}, {.361, .525, 1.44}, {.453, .809, 1.60}, {.592, .800, 2.00}, {.643, .542, 2.61}, {1.44, .995, 5.61}, {1.13, .826, 2.97}};
   const double bytes = (double)N * K;
   if (kind == 0) {
     const double turns = (K + 64 * kWaves * 4 - 1) / (64 * kWaves * 4), stream = bytes * (0.168e-6 + 0.00664e-6 * (M - 1));
@@ -490,7 +492,7 @@ inline double cost(int M, int N, int K, int kind, int splits) {
     const long whole = tiles / 256, rest = tiles % 256 * splits;
     t = whole * (stages * a + e) + (rest ? per * (b + (a - b) * rest / 256.) + e : 0);
     joined = 65536. * rest;
-  } else if (kind == 5) {
+  } else if (kind == 5 || kind == 7) {
     const long whole = tiles * splits / 256, rest = tiles * splits % 256;
     t = whole * (per * a + e) + (rest ? per * (b + (a - b) * rest / 256.) + e : 0);
   } else {
@@ -524,7 +526,7 @@ K8S_API int k8s_int8_gemm_plan(int M, int N, int K) {
   if (M <= 0 || N <= 0 || K <= 0) return 1 << 8;
   double best = 0;
   int plan = 0;
-  for (int kind = M <= 16 ? 0 : 1; kind < 7; ++kind)
+  for (int kind = M <= 16 ? 0 : 1; kind < 8; ++kind)
     for (int s : runs) {
       if (!can_cut(M, N, K, kind, s)) continue;
       const double t = cost(M, N, K, kind, s);
@@ -536,7 +538,7 @@ K8S_API int k8s_int8_gemm_plan(int M, int N, int K) {
 // int32 numbers of workspace that the plan needs
 K8S_API long k8s_int8_gemm_part(int M, int N, int kind, int splits) {
   using namespace k8s::q8;
-  if (splits <= 1 || kind < 0 || kind > 6) return 0;
+  if (splits <= 1 || kind < 0 || kind > 7) return 0;
   const long tiles = (long)((M - 1) / kEdge[kind][0] + 1) * ((N - 1) / kEdge[kind][1] + 1);
   return kind == 6 ? tiles % 256 * splits * 65536L : (long)splits * M * ((N + 7) / 8 * 8);
 }
@@ -547,7 +549,7 @@ K8S_API int k8s_int8_gemm(const void* x, long ldx, const float* xs, const void* 
                           long ldy, int f32, int M, int N, int K, int kind, int splits, void* part, long parts, void* stream) {
   using namespace k8s::q8;
   if (M <= 0 || N <= 0) return 0;
-  if (kind < 0 || kind > 6 || (kind == 0 && M > 16) || K <= 0 || (K & 15) || K > 131056 || splits < 1) return (int)hipErrorInvalidValue;
+  if (kind < 0 || kind > 7 || (kind == 0 && M > 16) || K <= 0 || (K & 15) || K > 131056 || splits < 1) return (int)hipErrorInvalidValue;
   if (!can_cut(M, N, K, kind, splits) || (splits > 1 && (!part || parts < k8s_int8_gemm_part(M, N, kind, splits)))) return (int)hipErrorInvalidValue;
   const int n_mt = (M - 1) / kEdge[kind][0] + 1, n_nt = (N - 1) / kEdge[kind][1] + 1;
   if ((long)n_mt * n_nt * splits > 0x7fffffffL || ((long)((N + 3) / 4) * M + 255) / 256 > 0x7fffffffL) return (int)hipErrorInvalidValue;
@@ -560,6 +562,7 @@ K8S_API int k8s_int8_gemm(const void* x, long ldx, const float* xs, const void* 
     case 3: ring<64, 128, 3, 4>(a, st); break;
     case 4: ring<128, 64, 3, 2>(a, st); break;
     case 5: ring<128, 128, 4, 4>(a, st); break;
+    case 7: ring<128, 256, 3, 8>(a, st); break;
     default: {
       // the tiles of whole rounds take all of K; those of the last, partial one are cut
       a.whole = splits > 1 ? n_mt * n_nt / 256 * 256 : n_mt * n_nt;

@@ -163,7 +163,7 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Op
 
 
 # ------------------------------------------------------------------ products
-FEW, T32, T64, T64_128, T128_64, T128, T256 = range(7)
+FEW, T32, T64, T64_128, T128_64, T128, T256, T128_256 = range(8)
 
 
 @lru_cache(maxsize=4096)

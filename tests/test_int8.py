@@ -209,6 +209,18 @@ def test_every_kernel_of_a_product(M, N, K, kind, runs, monkeypatch):
         check_product(Q.linear_int8(*args[:4], bias=args[4], out_dtype=dtype), *args)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(1, 3, 16), (50, 70, 400), (129, 257, 1040), (300, 515, 2064), (128, 256, 128), (257, 1288, 640)])
+@pytest.mark.parametrize("runs", [1, 3])
+def test_tiles_of_128_by_256(M, N, K, runs, monkeypatch):
+    stages = -(-K // 128)
+    runs = -(-stages // -(-stages // min(runs, stages)))       # (none of them empty)
+    forced(monkeypatch, Q.T128_256, runs)
+    for dtype in (BF, F32):
+        args = product_case("cuda", M, N, K, dtype, True)
+        check_product(Q.linear_int8(*args[:4], bias=args[4], out_dtype=dtype), *args)
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 1, 16), (3, 5, 48), (33, 17, 4096)])
 def test_product_plain(M, N, K):
     for dtype, bias in ((BF, False), (F32, True)):
