@@ -3,7 +3,7 @@
 // Tokens are rotated and written in one pass: q heads are rotated in place, a k head is rotated in fp32 and quantised from
 // there, a v head is quantised as it is.  What bounds it is memory: 8000 rows of 32 + 2 x 8 heads 47 us with
 // inputs from memory (181 MB: 3.9 TB/s), 40 us with one set of them that the caches hold in part (4.5 TB/s); rows of
-// many pages the single bytes of their values (1024 rows in as many pages 18 us).
+// many pages the single bytes of their values (1024 rows in as many pages 34 us).
 #include "int8_rows.h"
 
 namespace k8s {
@@ -100,11 +100,12 @@ __device__ __forceinline__ void rotate(const WriteArgs& a, int t, int part, int 
 }
 
 // Values of up to 64 rows of one head, turned in LDS: a dim's tokens lie side by side in a page, so that 16 rows whose slots
-// follow one another from a multiple of 16 on leave as 16 bytes a dim; others byte by byte.  Column c of a dim is row
-// c - (first row's slot mod 16), which lines the runs up.
+// follow one another from a multiple of 16 on leave as 16 bytes a dim; of others fours that do so as 4 bytes, the rest byte by
+// byte.  Column c of a dim is row c - (first row's slot mod 16), which lines the runs up.  us with the fours / without: 1055 rows of
+// 81 sequences, 16 + 2 x 16 heads, 14.5 / 21.5, 2652 of 22 17.1 / 22.4, 8000 of 5, 32 + 2 x 8 heads, 47.1 / 51.9.
 __device__ __forceinline__ void values(const WriteArgs& a, int t0, int head) {
   __shared__ uint8_t sm[128 * kPitch];
-  __shared__ int slots[kCols], whole[kCols / 16];
+  __shared__ int slots[kCols], whole[kCols / 16], piece[kCols];
   __shared__ size_t first[kCols];  // where the column's first dim lies in the cache
   const int tid = threadIdx.x, j = tid & 7;
   u16x8 in[kTokens / 32][2];
@@ -129,6 +130,13 @@ __device__ __forceinline__ void values(const WriteArgs& a, int t0, int head) {
     if (tid < kCols && (tid & 15) == 0) whole[tid >> 4] = ((run >> (tid & 63)) & 0xffff) == 0xffff;
   }
   __syncthreads();
+  if (tid < kCols) {  // bytes that leave from this column: four, if their slots are a whole piece of four, else its own, if no such piece has it
+    const int s = slots[tid], b = tid - (s & 3);
+    bool four = s >= 0 && b >= 0 && b + 3 < kCols;
+    if (four)
+      for (int e = 0; e < 4; ++e) four &= slots[b + e] == s - (s & 3) + e;
+    piece[tid] = s < 0 ? 0 : !four ? 1 : s & 3 ? 0 : 4;
+  }
 #pragma unroll
   for (int i = 0; i < kTokens / 32; ++i) {
     const int row = 32 * i + (tid >> 3);
@@ -158,13 +166,23 @@ __device__ __forceinline__ void values(const WriteArgs& a, int t0, int head) {
   __syncthreads();
   for (int i = tid; i < 128 * (kCols / 16); i += 256) {
     const int d = i / (kCols / 16), g = i % (kCols / 16);
-    if (whole[g]) {
-      const uint32_t* const p = reinterpret_cast<const uint32_t*>(sm + d * kPitch + 16 * g);
-      *reinterpret_cast<u32x4*>(a.v + first[16 * g] + (size_t)d * a.BS) = u32x4{p[0], p[1], p[2], p[3]};
-    } else {
+    if (!whole[g]) continue;
+    const uint32_t* const p = reinterpret_cast<const uint32_t*>(sm + d * kPitch + 16 * g);
+    *reinterpret_cast<u32x4*>(a.v + first[16 * g] + (size_t)d * a.BS) = u32x4{p[0], p[1], p[2], p[3]};
+  }
+  // (a lane a dim here: all lanes of a wave do the same)
+  for (int g = 0; g < kCols / 16; ++g) {
+    if (whole[g]) continue;
+    const int d = tid & 127, c0 = 16 * g + 8 * (tid >> 7);
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (slots[16 * g + e] >= 0) a.v[first[16 * g + e] + (size_t)d * a.BS] = sm[d * kPitch + 16 * g + e];
+    for (int e = 0; e < 8; ++e) {
+      const int n = __builtin_amdgcn_readfirstlane(piece[c0 + e]);
+      const uint8_t* const p = sm + d * kPitch + c0 + e;
+      uint8_t* const to = a.v + first[c0 + e] + (size_t)d * a.BS;
+      if (n == 4)
+        *reinterpret_cast<uint32_t*>(to) = pack4(p[0], p[1], p[2], p[3]);
+      else if (n)
+        *to = *p;
     }
   }
 }
@@ -189,10 +207,11 @@ K8S_API int k8s_int8_write(void* qkv, long ld, const int* pos, const float* cos_
   if (T <= 0) return 0;
   if (nq < 0 || nkv <= 0 || BS <= 0 || max_pos <= 0) return (int)hipErrorInvalidValue;
   const WriteArgs a{(uint16_t*)qkv, ld, pos, cos_sin, slots, (uint8_t*)k, (uint8_t*)v, ks, vs, T, nq, nkv, BS, max_pos, cap};
-  // The turn through LDS pays from some tokens and heads on.  us byte by byte / turned, rows whose slots follow one another: 32 + 2 x 8
-  // heads at 512 rows 7.0 / 8.5, 768 9.3 / 8.7, 8000 58.6 / 40.1; 8 + 2 x 1 heads at 4096 rows 8.1 / 9.2, 6000 10.6 / 10.1; 16 + 2 x
-  // 16 heads at 256 rows 7.3 / 8.1, 512 9.9 / 8.4.  Slots in as many pages: 32 + 2 x 8 heads at 1024 rows 18.5 / 17.7.
-  const bool turn = slots && (long)T * nkv >= 6000;
+  // The turn through LDS pays from some tokens and heads on.  us byte by byte / turned, rows of one sequence: 32 + 2 x 8 heads at 512 rows
+  // 7.9 / 7.7, 768 10.8 / 8.2; 8 + 2 x 1 heads at 4096 rows 9.7 / 8.8, 6000 12.3 / 10.0; 16 + 2 x 16 heads at 256 rows 7.5 / 6.9.  Of 13
+  // rows a sequence: 32 + 2 x 8 heads at 512 rows 9.8 / 10.3, 768 11.8 / 10.9; 8 + 2 x 1 heads at 4096 9.9 / 11.2; 16 + 2 x 16 heads
+  // at 128 rows 6.7 / 9.0, 400 11.2 / 9.9.  Of one row: 32 + 2 x 8 heads at 512 rows 11.2 / 13.8, 1024 34.8 / 34.8, 2000 82.5 / 75.2.
+  const bool turn = slots && (long)T * nkv >= 5000;
   // few tokens: a wave eight heads, so that no wave takes them one after another (one row of 32 + 2 x 8 heads 4.8 -> 3.3 us, 128 rows
   // 7.0 -> 4.2)
   const int eights = (nq + (turn || !slots ? 1 : 2) * nkv + 7) / 8, parts = T >= 2048 ? 1 : T * eights <= 2048 ? eights : 2048 / T;

@@ -341,6 +341,56 @@ def test_write(device, nq, nkv, BS, slots):
         assert torch.equal(t.transpose(1, 2)[rest], old.transpose(1, 2)[rest])
 
 
+def slots_of(kind, T, cap):
+    """T slots of a pool of cap: runs of several lengths at any alignment, with and without rows that are not kept."""
+    g = gen(T)
+    if kind == "shuffled":
+        return torch.randperm(cap, generator=g)[:T]
+    if kind == "backwards":
+        return torch.arange(cap - 3, cap - 3 - T, -1)
+    if kind == "one":
+        return torch.arange(5, 5 + T)
+    longest = {"short": 9, "threads": 41, "gaps": 30}[kind]
+    out, at = [], 0
+    while len(out) < T:
+        at += int(torch.randint(0, 7, (1,), generator=g))
+        n = int(torch.randint(1, longest + 1, (1,), generator=g))
+        out += range(at, at + n)
+        at += n
+    out = torch.tensor(out[:T])
+    assert int(out.max()) < cap
+    if kind == "gaps":
+        out[torch.rand(T, generator=g) < 0.05] = -1
+        out[T // 2] = cap
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["shuffled", "backwards", "one", "short", "threads", "gaps"])
+@pytest.mark.parametrize("T,nq,nkv,BS", [(700, 16, 16, 64), (2513, 4, 2, 192), (5001, 1, 1, 128)])
+def test_write_of_many_rows(kind, T, nq, nkv, BS):
+    cap = (3 * T + 200) // BS * BS
+    slots = slots_of(kind, T, cap)
+    qkv, pos, at = write_case(T, nq, nkv, BS, slots)
+    cs = table(512)
+    cache = noise(Q.Int8KV.empty(cap // BS, nkv, BS, "cuda"))
+    want = Q.Int8KV(*(t.clone().cpu() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)))
+    mine = qkv.cuda()
+    Q.rope_kv_write_int8(mine, pos.cuda(), cs.cuda(), at.cuda(), cache, nq, nkv)
+    Q.rope_kv_write_int8(qkv, pos, cs, at, want, nq, nkv)
+    assert torch.equal(cache.v.cpu(), want.v) and bool(((cache.v_scale.cpu() - want.v_scale).abs() <= 2.0 ** -23 * want.v_scale).all())
+    # (a rotated key's last bit may differ, and an integer half way between two with it)
+    off = (cache.k.cpu().int() - want.k.int()).abs()
+    assert int(off.max()) <= 1 and float((off > 0).double().mean()) < 1e-3
+    assert bool(((cache.k_scale.cpu() - want.k_scale).abs() <= 2.0 ** -21 * want.k_scale).all())
+    kept = (slots >= 0) & (slots < cap)
+    rest = torch.ones(cap, dtype=torch.bool)
+    rest[slots[kept]] = False
+    rest = rest.view(-1, BS)
+    assert torch.equal(cache.k.cpu().transpose(1, 2)[rest], want.k.transpose(1, 2)[rest])
+    assert torch.equal(cache.k_scale.cpu().transpose(1, 2)[rest], want.k_scale.transpose(1, 2)[rest])
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_write_without_slots_and_without_rows(device):
     qkv, pos, _ = write_case(3, 4, 2, 64, [0, 1, 2])
