@@ -1,8 +1,8 @@
 // A paged cache of keys and values in 8 bits, one scale a token and head (int8_rows.h):
 //   k [blocks][nkv][BS][128], v [blocks][nkv][128][BS] (transposed pages, as in the bf16 cache), scales [blocks][nkv][BS].
 // Tokens are rotated and written in one pass: q heads are rotated in place, a k head is rotated in fp32 and quantised from
-// there, a v head is quantised as it is.  What bounds it is memory: 8000 rows of 32 + 2 x 8 heads 47 us with
-// inputs from memory (181 MB: 3.9 TB/s), 40 us with one set of them that the caches hold in part (4.5 TB/s); rows of
+// there, a v head is quantised as it is.  What bounds it is memory: 8000 rows of 32 + 2 x 8 heads 43 us
+// (five sequences; 181 MB: 4.2 TB/s); rows of
 // many pages the single bytes of their values (1024 rows in as many pages 34 us).
 #include "int8_rows.h"
 
