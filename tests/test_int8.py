@@ -585,6 +585,18 @@ def test_chunk(device, lens, nq, nkv, BS):
     check_attention(out, q, cache, meta, starts, ctx, nq, nkv, 0.09)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,nq,nkv,BS", [([(1, 9000), (1, 4097)], 8, 2, 64), ([(5, 9000)], 8, 2, 64), ([(300, 9000), (70, 4161)], 8, 2, 64),
+                                            ([(2, 8300), (130, 130)], 10, 2, 64), ([(40, 9001)], 4, 4, 256)])
+def test_whole_key_ranges_of_more_than_64_pages(lens, nq, nkv, BS):
+    q, cache, meta, starts, ctx = attn_case("cuda", lens, nq, nkv, BS)
+    if meta.decode:
+        planned(meta, starts, ctx, nq, nkv, BS, part=16384)
+    else:
+        A.attach_plan(meta, A.plan_prefill(starts, nq // nkv, BS), "cuda")
+    check_attention(Q.paged_attention_int8(q, cache, meta, nq, nkv, 0.09), q, cache, meta, starts, ctx, nq, nkv, 0.09)
+
+
 # heads and pages whose tiles the kernel finds by itself: keys cut and whole, sequences without rows, with fewer keys than rows and in
 # more groups of 64 than one, a table wider than any context
 OWN = [([(6, 2000), (0, 500), (3, 3)], 10, 2, 64, 0), ([(1, 1)] + [(0, 70)] * 70 + [(2, 130), (60, 60)], 12, 4, 64, 0), ([(400, 900)], 10, 10, 128, 0),
