@@ -325,8 +325,7 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
         raise ValueError("block_tables must be int32 [S, pages]")
     if S > 1 and bt.stride(0) < bt.shape[1]:
         raise ValueError("the rows of block_tables overlap")
-    if ctx.dtype != torch.int32 or starts.dtype != torch.int32 or ctx.numel() < S or starts.numel() < S + 1:
-        raise ValueError("ctx_lens must be int32 [S] and q_start int32 [S + 1]")
+    ctx, starts = _lengths(ctx, starts, S)
     ldq = _pitch(q)
     if not ldq:
         raise ValueError("q's rows must be dense and start at multiples of 16 bytes")
@@ -373,6 +372,13 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
           ptr(meta.tile_len), ptr(meta.tile_kv0), ptr(meta.tile_kv1), ptr(meta.tile_slot), tiles, rows, ptr(meta.m_tok0),
           ptr(meta.m_len), ptr(meta.m_slot0), ptr(meta.m_np), merged, ptr(part_o), ptr(part_ml), A.PF8_ROWS, own, runs)
     return out
+
+
+def _lengths(ctx: torch.Tensor, starts: torch.Tensor, S: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """ctx_lens and q_start as the kernels read them: one behind another (a column of a wider table is copied)."""
+    if ctx.dtype != torch.int32 or starts.dtype != torch.int32 or ctx.dim() != 1 or starts.dim() != 1 or ctx.numel() < S or starts.numel() < S + 1:
+        raise ValueError("ctx_lens must be int32 [S] and q_start int32 [S + 1]")
+    return ctx.contiguous(), starts.contiguous()
 
 
 def _planned(dev: int, *arrays) -> None:

@@ -692,6 +692,36 @@ def test_pages_behind_two_gigabytes():
         del far
 
 
+def columns(meta):
+    """The same lengths and starts as columns of wider tables, whose other columns say something else."""
+    wide = lambda t: torch.stack([t, 3 * t + 5], 1)[:, 0]  # noqa: E731
+    meta.ctx_lens, meta.q_start = wide(meta.ctx_lens), wide(meta.q_start)
+    assert not meta.ctx_lens.is_contiguous() or meta.ctx_lens.numel() == 1
+    return meta
+
+
+def test_lengths_are_read_one_behind_another():
+    _, _, meta, starts, ctx = attn_case("cpu", [(1, 300), (1, 0), (1, 65)], 4, 2)
+    columns(meta)
+    a, b = Q._lengths(meta.ctx_lens, meta.q_start, 3)
+    assert a.is_contiguous() and b.is_contiguous() and a.tolist() == ctx and b.tolist() == starts
+    for bad in ((meta.ctx_lens.long(), meta.q_start), (meta.ctx_lens[:2], meta.q_start), (meta.ctx_lens, meta.q_start[:3]),
+                (meta.ctx_lens[:, None], meta.q_start), (meta.ctx_lens, meta.q_start.float())):
+        with pytest.raises(ValueError):
+            Q._lengths(*bad, 3)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lens,nq,nkv", [([(1, 700), (1, 0), (1, 129), (1, 1)], 8, 2), ([(5, 90), (0, 70), (64, 64), (3, 200)], 8, 2),
+                                         ([(5, 90), (0, 70), (64, 64), (3, 200)], 10, 2)])
+def test_lengths_in_columns_of_wider_tables(device, lens, nq, nkv):
+    q, cache, meta, starts, ctx = attn_case(device, lens, nq, nkv)
+    if device == "cuda":
+        planned(meta, starts, ctx, nq, nkv, 64)
+    out = Q.paged_attention_int8(q, cache, columns(meta), nq, nkv, 0.09)
+    check_attention(out, q, cache, meta, starts, ctx, nq, nkv, 0.09)
+
+
 # ------------------------------------------------------------------ refusals
 def test_refusals():
     x, w = torch.randn(4, 64), torch.ones(64)
