@@ -177,6 +177,7 @@ class AttnMeta:
     m_slot0: Optional[torch.Tensor] = None
     m_np: Optional[torch.Tensor] = None
     n_merge: int = 0
+    n_slots: int = 0                          # partial-result slots that the plan uses; 0: not said
     pf_o: Optional[torch.Tensor] = None
     pf_ml: Optional[torch.Tensor] = None
     # decode split-KV
@@ -565,6 +566,7 @@ def attach_plan(meta: "AttnMeta", plan: PrefillPlan, device, workspace: Optional
     (meta.tile_seq, meta.tile_tok0, meta.tile_len, meta.tile_kv0, meta.tile_kv1, meta.tile_slot,
      meta.m_tok0, meta.m_len, meta.m_slot0, meta.m_np) = t
     meta.n_tiles, meta.n_merge = plan.n_tiles, plan.n_merge
+    meta.n_slots = max(plan.slot, default=-1) + 1
     if workspace is not None:
         meta.pf_o, meta.pf_ml = workspace
     return meta

@@ -340,8 +340,8 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
         if meta.items is None or meta.items.dtype != torch.int32:
             raise ValueError("the step has no plan: attach_decode_plan")
         _planned(dev, meta.items, meta.d_n_items, meta.part_o, meta.part_ml)
-        if meta.n_parts > 1 and meta.part_o is None:
-            raise ValueError("a plan of several parts needs part_o and part_ml")
+        if meta.n_parts > 1 and not _room(meta.part_o, meta.part_ml, S * nq * meta.n_parts):
+            raise ValueError(f"a plan of several parts needs part_o and part_ml of {S} x {nq} x {meta.n_parts} rows")
         grid = max(1, meta.grid_waves or min(A.DECODE_WAVE_SLOTS, meta.n_items * nkv))
         _call("k8s_int8_attn_reply", dev, *common, S, nq, nkv, BS, scale, out.data_ptr(), ldo, ptr(meta.part_o), ptr(meta.part_ml),
               meta.n_parts, meta.part_size, meta.items.data_ptr(), meta.n_items, ptr(meta.d_n_items), grid)
@@ -364,10 +364,11 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
         tiles, merged, rows = T // own + S, 0, own * G
         blocks, pages = tiles * nkv, bt.shape[1] * BS // 64
         runs = max(1, min(256 // blocks, pages // 5) if blocks <= 128 else min(512 // blocks, pages // 16))
-        part_o = None
-    if part_o is None and (merged or runs > 1):  # (a split tile's parts are tiles of the plan: no more than those, without a look at the device)
-        part_o = scratch(tiles * runs * nkv * A.PF8_ROWS * D, torch.float32, q.device)
-        part_ml = scratch(tiles * runs * nkv * A.PF8_ROWS * 2, torch.float32, q.device)
+    if merged or runs > 1:  # (a split tile's parts are tiles of the plan: no more than those, without a look at the device)
+        rows_kept = (tiles * runs if own else meta.n_slots or tiles) * nkv * A.PF8_ROWS
+        if own or not _room(part_o, part_ml, rows_kept):  # (none in the plan, or one for fewer key heads)
+            part_o = scratch(rows_kept * D, torch.float32, q.device)
+            part_ml = scratch(rows_kept * 2, torch.float32, q.device)
     _call("k8s_int8_attn_chunk", dev, *common, S, nq, nkv, BS, scale, out.data_ptr(), ldo, ptr(meta.tile_seq), ptr(meta.tile_tok0),
           ptr(meta.tile_len), ptr(meta.tile_kv0), ptr(meta.tile_kv1), ptr(meta.tile_slot), tiles, rows, ptr(meta.m_tok0),
           ptr(meta.m_len), ptr(meta.m_slot0), ptr(meta.m_np), merged, ptr(part_o), ptr(part_ml), A.PF8_ROWS, own, runs)
@@ -379,6 +380,12 @@ def _lengths(ctx: torch.Tensor, starts: torch.Tensor, S: int) -> Tuple[torch.Ten
     if ctx.dtype != torch.int32 or starts.dtype != torch.int32 or ctx.dim() != 1 or starts.dim() != 1 or ctx.numel() < S or starts.numel() < S + 1:
         raise ValueError("ctx_lens must be int32 [S] and q_start int32 [S + 1]")
     return ctx.contiguous(), starts.contiguous()
+
+
+def _room(part_o: Optional[torch.Tensor], part_ml: Optional[torch.Tensor], rows: int) -> bool:
+    """Whether a plan's workspace holds the parts of so many rows: O, and its maximum and sum."""
+    return part_o is not None and part_ml is not None and all(
+        t.dtype == torch.float32 and t.is_contiguous() and t.numel() >= rows * n for t, n in ((part_o, HEAD_DIM), (part_ml, 2)))
 
 
 def _planned(dev: int, *arrays) -> None:

@@ -722,6 +722,46 @@ def test_lengths_in_columns_of_wider_tables(device, lens, nq, nkv):
     check_attention(out, q, cache, meta, starts, ctx, nq, nkv, 0.09)
 
 
+def test_room_of_a_plan():
+    o, ml = torch.empty(3 * 8 * 4 * D), torch.empty(3 * 8 * 4 * 2)
+    assert Q._room(o, ml, 96) and Q._room(o.view(-1, D), ml, 95)
+    assert not Q._room(o, ml, 97) and not Q._room(None, ml, 1) and not Q._room(o, None, 1) and not Q._room(o[:-1], ml, 96)
+    assert not Q._room(o, ml[:-1], 96) and not Q._room(o.to(BF), ml, 1) and not Q._room(o[::2], ml, 1)
+    _, _, meta, starts, ctx = attn_case("cpu", [(70, 3000), (3, 9)], 8, 2)
+    plan = A.plan_prefill(starts, 4, 64, ctx, 2)
+    A.attach_plan(meta, plan, "cpu")
+    assert plan.n_merge and meta.n_slots == sum(plan.m_np) == meta.m_slot0_end()
+
+
+@pytest.mark.gpu
+def test_a_reply_plan_for_fewer_heads_is_refused():
+    q, cache, meta, starts, ctx = attn_case("cuda", [(1, 900), (1, 300)], 32, 8)
+    planned(meta, starts, ctx, 8, 2, 64, part=64)
+    with pytest.raises(ValueError):
+        Q.paged_attention_int8(q, cache, meta, 32, 8, 0.09)
+    planned(meta, starts, ctx, 32, 8, 64, part=64)
+    meta.part_ml = meta.part_ml[:-1]
+    with pytest.raises(ValueError):
+        Q.paged_attention_int8(q, cache, meta, 32, 8, 0.09)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("said", [True, False])
+def test_a_chunk_takes_room_of_its_own_where_the_plan_has_too_little(said):
+    q, cache, meta, starts, ctx = attn_case("cuda", [(70, 3000)], 16, 4)
+    planned(meta, starts, ctx, 16, 4, 64)
+    meta.pf_o, meta.pf_ml = A.prefill_workspace(1, "cuda", meta.n_slots)
+    meta.pf_o.fill_(7.0)
+    if not said:
+        meta.n_slots = 0
+    check_attention(Q.paged_attention_int8(q, cache, meta, 16, 4, 0.09), q, cache, meta, starts, ctx, 16, 4, 0.09)
+    assert bool((meta.pf_o == 7).all())
+    meta.pf_o, meta.pf_ml = A.prefill_workspace(4, "cuda", meta.n_tiles)
+    meta.pf_o.fill_(7.0)
+    check_attention(Q.paged_attention_int8(q, cache, meta, 16, 4, 0.09), q, cache, meta, starts, ctx, 16, 4, 0.09)
+    assert not bool((meta.pf_o == 7).all())
+
+
 # ------------------------------------------------------------------ refusals
 def test_refusals():
     x, w = torch.randn(4, 64), torch.ones(64)
