@@ -34,7 +34,7 @@ struct AttnArgs {
   // replies: a list of (row, part | -1, end key, q row | (tokens - 1) << 24), parts of part_size keys
   const int4* items;
   int n_items;
-  const int* d_items;  // {items, keys a part} on the device, or null
+  const int* d_items;  // {items, keys a part} on the device, of n_items that the list has room for; or null
   float *part_o, *part_ml;
   int n_parts, part_size;
   // chunks: tiles of rows and runs of 64-key pages
@@ -205,7 +205,7 @@ __device__ __forceinline__ void put_part(const State& st, int i, float m, float 
 // ------------------------------------------------------------------ replies
 __global__ void __launch_bounds__(64, 2) reply_kernel(AttnArgs a) {
   const int lane = threadIdx.x, r = lane & 15, g = lane >> 4;
-  const int n_items = a.d_items ? __builtin_amdgcn_readfirstlane(a.d_items[0]) : a.n_items;
+  const int n_items = a.d_items ? min(__builtin_amdgcn_readfirstlane(a.d_items[0]), a.n_items) : a.n_items;
   const int part_size = a.d_items ? __builtin_amdgcn_readfirstlane(a.d_items[1]) : a.part_size;
   const int total = n_items * a.nkv;
   for (int w = blockIdx.x; w < total; w += gridDim.x) {
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(64, 2) reply_kernel(AttnArgs a) {
       const int ti = row / a.G, head = kvh * a.G + row - ti * a.G;
       if (whole) {
         put_row(st, i, l[i] == 0.f ? 0.f : 1.f / l[i], a.out + (qrow + ti) * a.ldo + head * D, r);
-      } else {
+      } else if (a.n_parts > 1 && part < a.n_parts) {  // (else there is no room for it)
         const size_t at = ((size_t)(seq + ti) * a.nq + head) * a.n_parts + part;
         put_part(st, i, m[i], l[i], a.part_o + at * D, a.part_ml + at * 2, r);
       }

@@ -337,22 +337,28 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
             raise ValueError(f"a reply step has one row a sequence, not {T} for {S}")
         if G > 16:
             raise ValueError(f"{G} query heads a key head: a reply step takes 16")
-        if meta.items is None or meta.items.dtype != torch.int32:
+        if meta.items is None:
             raise ValueError("the step has no plan: attach_decode_plan")
-        _planned(dev, meta.items, meta.d_n_items, meta.part_o, meta.part_ml)
+        _on(dev, meta.part_o, meta.part_ml)
+        _listed(dev, 4 * meta.n_items, meta.items)
+        n_items = meta.n_items
+        if meta.d_n_items is not None:
+            _listed(dev, 2, meta.d_n_items)
+            n_items = meta.items.numel() // 4  # (the count that the device reads goes no further)
         if meta.n_parts > 1 and not _room(meta.part_o, meta.part_ml, S * nq * meta.n_parts):
             raise ValueError(f"a plan of several parts needs part_o and part_ml of {S} x {nq} x {meta.n_parts} rows")
         grid = max(1, meta.grid_waves or min(A.DECODE_WAVE_SLOTS, meta.n_items * nkv))
         _call("k8s_int8_attn_reply", dev, *common, S, nq, nkv, BS, scale, out.data_ptr(), ldo, ptr(meta.part_o), ptr(meta.part_ml),
-              meta.n_parts, meta.part_size, meta.items.data_ptr(), meta.n_items, ptr(meta.d_n_items), grid)
+              meta.n_parts, meta.part_size, meta.items.data_ptr(), n_items, ptr(meta.d_n_items), grid)
         return out
     rows = A.prefill_tile_tokens(G, BS) * G
     if rows > A.PF8_ROWS:
         raise ValueError(f"{G} query heads a key head: a tile takes {A.PF8_ROWS}")
     if meta.tile_seq is None or meta.tile_kv1 is None:
         raise ValueError("the step has no plan: attach_plan")
-    _planned(dev, meta.tile_seq, meta.tile_tok0, meta.tile_len, meta.tile_kv0, meta.tile_kv1, meta.tile_slot, meta.m_tok0, meta.m_len, meta.m_slot0,
-             meta.m_np, meta.pf_o, meta.pf_ml)
+    _on(dev, meta.pf_o, meta.pf_ml)
+    _listed(dev, meta.n_tiles, meta.tile_seq, meta.tile_tok0, meta.tile_len, meta.tile_kv0, meta.tile_kv1, meta.tile_slot)
+    _listed(dev, meta.n_merge, meta.m_tok0, meta.m_len, meta.m_slot0, meta.m_np)
     part_o, part_ml, tiles, merged, own, runs = meta.pf_o, meta.pf_ml, meta.n_tiles, meta.n_merge, 0, 1
     if A.PF_ROWS % G or BS != 64:
         # Where heads or pages do not fit the bf16 cache's kernels the plan has tiles of about 64 rows over whole key ranges.  A workgroup
@@ -388,10 +394,23 @@ def _room(part_o: Optional[torch.Tensor], part_ml: Optional[torch.Tensor], rows:
         t.dtype == torch.float32 and t.is_contiguous() and t.numel() >= rows * n for t, n in ((part_o, HEAD_DIM), (part_ml, 2)))
 
 
-def _planned(dev: int, *arrays) -> None:
-    for t in arrays:
+def _on(dev: int, *tensors) -> None:
+    for t in tensors:
         if t is not None and t.get_device() != dev:
             raise ValueError(f"a plan on {t.device} for device {dev}")
+
+
+def _listed(dev: int, n: int, *lists) -> None:
+    """A plan's lists: what the kernels read of them is there, one behind another."""
+    for t in lists:
+        if t is None:
+            if n > 0:
+                raise ValueError("a list of the step's plan is missing")
+            continue
+        if t.get_device() != dev:
+            _on(dev, t)
+        if t.dtype != torch.int32 or t.numel() < n or not t.is_contiguous():
+            raise ValueError(f"a plan's list must be contiguous int32 of {n}, not {t.dtype} {list(t.shape)}")
 
 
 def _attention_plain(q, cache: Int8KV, meta: A.AttnMeta, nq, nkv, scale, out):

@@ -762,6 +762,41 @@ def test_a_chunk_takes_room_of_its_own_where_the_plan_has_too_little(said):
     assert not bool((meta.pf_o == 7).all())
 
 
+def test_lists_of_a_plan():
+    n = torch.arange(12, dtype=torch.int32)
+    Q._listed(-1, 12, n, n.view(3, 4))
+    Q._listed(-1, 0, n, None)
+    Q._listed(-1, 6, n[6:])
+    for count, t in ((13, n), (6, n[::2]), (4, n.long()), (4, n.float()), (1, None)):
+        with pytest.raises(ValueError):
+            Q._listed(-1, count, n, t)
+    with pytest.raises(ValueError):
+        Q._listed(0, 1, n)
+
+
+@pytest.mark.gpu
+def test_a_plan_with_lists_that_are_not_the_kernels_is_refused():
+    q, cache, meta, starts, ctx = attn_case("cuda", [(1, 900), (1, 300)], 8, 2)
+    planned(meta, starts, ctx, 8, 2, 64, part=64)
+    items, n = meta.items, meta.n_items
+    for meta.items, meta.n_items in ((items[:-1], n), (items, n + 1), (torch.stack([items, items], 2)[..., 0], n), (items.long(), n)):
+        with pytest.raises(ValueError):
+            Q.paged_attention_int8(q, cache, meta, 8, 2, 0.09)
+    meta.items, meta.n_items, meta.d_n_items = items, n, torch.tensor([n], dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        Q.paged_attention_int8(q, cache, meta, 8, 2, 0.09)
+    meta.d_n_items = torch.tensor([n + 1000, 64], dtype=torch.int32, device="cuda")   # (more than the list has: it ends where it ends)
+    check_attention(Q.paged_attention_int8(q, cache, meta, 8, 2, 0.09), q, cache, meta, starts, ctx, 8, 2, 0.09)
+    for what in ("tile_seq", "tile_kv1", "m_slot0"):
+        q, cache, meta, starts, ctx = attn_case("cuda", [(70, 3000)], 8, 2)
+        planned(meta, starts, ctx, 8, 2, 64)
+        whole = getattr(meta, what)
+        for part in (whole[:-1], whole.long(), None, torch.stack([whole, whole], 1)[:, 0] if whole.numel() > 1 else whole[:0]):
+            setattr(meta, what, part)
+            with pytest.raises(ValueError):
+                Q.paged_attention_int8(q, cache, meta, 8, 2, 0.09)
+
+
 # ------------------------------------------------------------------ refusals
 def test_refusals():
     x, w = torch.randn(4, 64), torch.ones(64)
