@@ -358,7 +358,8 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
         raise ValueError("the step has no plan: attach_plan")
     _on(dev, meta.pf_o, meta.pf_ml)
     _listed(dev, meta.n_tiles, meta.tile_seq, meta.tile_tok0, meta.tile_len, meta.tile_kv0, meta.tile_kv1, meta.tile_slot)
-    _listed(dev, meta.n_merge, meta.m_tok0, meta.m_len, meta.m_slot0, meta.m_np)
+    if meta.n_merge:
+        _listed(dev, meta.n_merge, meta.m_tok0, meta.m_len, meta.m_slot0, meta.m_np)
     part_o, part_ml, tiles, merged, own, runs = meta.pf_o, meta.pf_ml, meta.n_tiles, meta.n_merge, 0, 1
     if A.PF_ROWS % G or BS != 64:
         # Where heads or pages do not fit the bf16 cache's kernels the plan has tiles of about 64 rows over whole key ranges.  A workgroup
@@ -390,8 +391,8 @@ def _lengths(ctx: torch.Tensor, starts: torch.Tensor, S: int) -> Tuple[torch.Ten
 
 def _room(part_o: Optional[torch.Tensor], part_ml: Optional[torch.Tensor], rows: int) -> bool:
     """Whether a plan's workspace holds the parts of so many rows: O, and its maximum and sum."""
-    return part_o is not None and part_ml is not None and all(
-        t.dtype == torch.float32 and t.is_contiguous() and t.numel() >= rows * n for t, n in ((part_o, HEAD_DIM), (part_ml, 2)))
+    return (part_o is not None and part_ml is not None and part_o.dtype is torch.float32 and part_ml.dtype is torch.float32
+            and part_o.numel() >= HEAD_DIM * rows and part_ml.numel() >= 2 * rows and part_o.is_contiguous() and part_ml.is_contiguous())
 
 
 def _on(dev: int, *tensors) -> None:
@@ -409,7 +410,7 @@ def _listed(dev: int, n: int, *lists) -> None:
             continue
         if t.get_device() != dev:
             _on(dev, t)
-        if t.dtype != torch.int32 or t.numel() < n or not t.is_contiguous():
+        if t.dtype is not torch.int32 or t.numel() < n or not t.is_contiguous():
             raise ValueError(f"a plan's list must be contiguous int32 of {n}, not {t.dtype} {list(t.shape)}")
 
 
