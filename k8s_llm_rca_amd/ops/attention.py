@@ -178,6 +178,7 @@ class AttnMeta:
     m_np: Optional[torch.Tensor] = None
     n_merge: int = 0
     n_slots: int = 0                          # partial-result slots that the plan uses; 0: not said
+    tile_tokens: int = 0                      # tokens of its longest tile; 0: not said
     pf_o: Optional[torch.Tensor] = None
     pf_ml: Optional[torch.Tensor] = None
     # decode split-KV
@@ -188,6 +189,7 @@ class AttnMeta:
     # decode work list (persistent kernel, BS % 64 == 0): see build_decode_items
     items: Optional[torch.Tensor] = None      # [n_items, 4] int32
     n_items: int = 0
+    item_tokens: int = 0                      # most tokens that share an item; 0: not said
     d_n_items: Optional[torch.Tensor] = None  # [2] int32 device {item count, part_size} (HIP graphs)
     grid_waves: int = 0
     # host copies for the reference path
@@ -304,6 +306,7 @@ def attach_decode_plan(meta: "AttnMeta", ctx_host, nq: int, nkv: int, block_size
                                    max(1, 16 // G) if G <= 16 else 1)
         meta.items = torch.from_numpy(items).to(device)
         meta.n_items = items.shape[0]
+        meta.item_tokens = int((items[:, 3] >> 24).max(initial=0)) + 1
     else:
         P = part or 512
         n = max(1, -(-max(ctx_host) // P))
@@ -567,6 +570,7 @@ def attach_plan(meta: "AttnMeta", plan: PrefillPlan, device, workspace: Optional
      meta.m_tok0, meta.m_len, meta.m_slot0, meta.m_np) = t
     meta.n_tiles, meta.n_merge = plan.n_tiles, plan.n_merge
     meta.n_slots = max(plan.slot, default=-1) + 1
+    meta.tile_tokens = max(plan.length, default=0)
     if workspace is not None:
         meta.pf_o, meta.pf_ml = workspace
     return meta

@@ -345,6 +345,8 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
         if meta.d_n_items is not None:
             _listed(dev, 2, meta.d_n_items)
             n_items = meta.items.numel() // 4  # (the count that the device reads goes no further)
+        if meta.item_tokens * G > 16:
+            raise ValueError(f"a plan whose items have {meta.item_tokens} tokens, for fewer than {G} query heads a key head")
         if meta.n_parts > 1 and not _room(meta.part_o, meta.part_ml, S * nq * meta.n_parts):
             raise ValueError(f"a plan of several parts needs part_o and part_ml of {S} x {nq} x {meta.n_parts} rows")
         grid = max(1, meta.grid_waves or min(A.DECODE_WAVE_SLOTS, meta.n_items * nkv))
@@ -371,6 +373,8 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
         tiles, merged, rows = T // own + S, 0, own * G
         blocks, pages = tiles * nkv, bt.shape[1] * BS // 64
         runs = max(1, min(256 // blocks, pages // 5) if blocks <= 128 else min(512 // blocks, pages // 16))
+    elif meta.tile_tokens * G > A.PF8_ROWS:
+        raise ValueError(f"a plan whose tiles have {meta.tile_tokens} tokens, for fewer than {G} query heads a key head")
     if merged or runs > 1:  # (a split tile's parts are tiles of the plan: no more than those, without a look at the device)
         rows_kept = (tiles * runs if own else meta.n_slots or tiles) * nkv * A.PF8_ROWS
         if own or not _room(part_o, part_ml, rows_kept):  # (none in the plan, or one for fewer key heads)

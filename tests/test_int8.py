@@ -797,6 +797,50 @@ def test_a_plan_with_lists_that_are_not_the_kernels_is_refused():
                 Q.paged_attention_int8(q, cache, meta, 8, 2, 0.09)
 
 
+def chained(nq, nkv, device):
+    """Seven tokens of one sequence as rows of a reply step that share items, as many as so many heads let them."""
+    q, cache, meta, starts, ctx = attn_case(device, [(1, 700)], nq, nkv)
+    lens = [694 + i for i in range(7)]
+    meta = A.AttnMeta(block_tables=meta.block_tables.expand(7, -1).contiguous(), ctx_lens=torch.tensor(lens, dtype=torch.int32, device=device),
+                      q_start=torch.arange(8, dtype=torch.int32, device=device), num_seqs=7, decode=True)
+    return cache, meta, lens
+
+
+def test_a_plan_says_how_many_tokens_share_an_item_or_a_tile():
+    for nq, nkv, most in ((8, 2, 4), (8, 8, 7), (32, 2, 1), (10, 2, 3)):
+        _, meta, lens = chained(nq, nkv, "cpu")
+        A.attach_decode_plan(meta, lens, nq, nkv, 64, "cpu", part=2048, chain=[False] + [True] * 6)
+        assert meta.item_tokens == most
+        A.attach_decode_plan(meta, lens, nq, nkv, 64, "cpu")
+        assert meta.item_tokens == 1
+    _, _, meta, starts, ctx = attn_case("cpu", [(70, 3000), (300, 300)], 8, 2)
+    A.attach_plan(meta, A.plan_prefill(starts, 4, 64, ctx, 2), "cpu")
+    assert meta.tile_tokens == 64
+    A.attach_plan(meta, A.plan_prefill([0, 5, 9], 4, 64, [5, 9], 2), "cpu")
+    assert meta.tile_tokens == 5
+
+
+@pytest.mark.gpu
+def test_a_plan_for_fewer_query_heads_a_key_head_is_refused():
+    """Its items and tiles hold more rows than a wave or a workgroup, which would leave the last ones out."""
+    for plan_nq, nq in ((8, 8), (16, 8), (8, 16), (8, 32)):
+        cache, meta, lens = chained(nq, 4, "cuda")
+        q = randn(gen(5), 7, nq * D, dtype=BF, device="cuda")
+        A.attach_decode_plan(meta, lens, plan_nq, 4, 64, "cuda", part=2048, chain=[False] + [True] * 6)
+        if nq > plan_nq:
+            with pytest.raises(ValueError):
+                Q.paged_attention_int8(q, cache, meta, nq, 4, 0.09)
+        else:
+            check_attention(Q.paged_attention_int8(q, cache, meta, nq, 4, 0.09), q, cache, meta, list(range(8)), lens, nq, 4, 0.09)
+    q, cache, meta, starts, ctx = attn_case("cuda", [(70, 300), (300, 300)], 16, 2)
+    planned(meta, starts, ctx, 4, 2, 64)
+    with pytest.raises(ValueError):
+        Q.paged_attention_int8(q, cache, meta, 16, 2, 0.09)
+    q, cache, meta, starts, ctx = attn_case("cuda", [(9, 300), (3, 300)], 16, 2)               # (tiles as long as both plans make them)
+    planned(meta, starts, ctx, 4, 2, 64)
+    check_attention(Q.paged_attention_int8(q, cache, meta, 16, 2, 0.09), q, cache, meta, starts, ctx, 16, 2, 0.09)
+
+
 # ------------------------------------------------------------------ refusals
 def test_refusals():
     x, w = torch.randn(4, 64), torch.ones(64)
