@@ -11,6 +11,8 @@
 // row rho of key tile (u, t) is key 16 (rho >> 2) + 8 u + 4 t + (rho & 3), so that lane group g = lane >> 4 is left with the
 // scores of keys 16 g .. 16 g + 15, whose values of one dim are one 16-byte load, and weights go to the second product
 // without leaving their lane.  Dims of K and Q are taken as 64 c + 16 g + [0, 16) by lane group g: one 16-byte load, two steps.
+#include <algorithm>
+
 #include "int8_rows.h"
 
 namespace k8s {
@@ -25,7 +27,8 @@ struct AttnArgs {
   const uint8_t *k, *v;
   const float *ks, *vs;
   const int* bt;       // [S][bt_stride] block ids
-  int bt_stride, NB;   // (a context behind the table's end, a page outside the pool: clamped, never read)
+  int bt_stride, NB;
+  int bt_keys;         // what a row of the table has pages for (a context behind that, a page outside the pool: clamped, never read)
   const int *ctx, *q_start;
   int S, nq, nkv, G, BS;
   float scale_log2;
@@ -211,7 +214,7 @@ __global__ void __launch_bounds__(64, 2) reply_kernel(AttnArgs a) {
   for (int w = blockIdx.x; w < total; w += gridDim.x) {
     const int it = w / a.nkv, kvh = w - it * a.nkv;
     const int4 item = a.items[it];
-    const int seq = item.x, k1 = min(item.z, a.bt_stride * a.BS), qrow = item.w & 0xFFFFFF, nt = (item.w >> 24) + 1;
+    const int seq = item.x, k1 = min(item.z, a.bt_keys), qrow = item.w & 0xFFFFFF, nt = (item.w >> 24) + 1;
     const bool whole = item.y < 0;
     const int part = whole ? 0 : item.y, k0 = part * part_size;
     const int qi = r / a.G;
@@ -372,7 +375,7 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(AttnArgs a) {
   const int* const bt = a.bt + (size_t)seq * a.bt_stride;
   const int grow = 32 * w + r;
   const bool valid = grow < rows;
-  const int end = min(base + len, a.bt_stride * a.BS);      // keys of the whole tile
+  const int end = min(base + len, a.bt_keys);               // keys of the whole tile
   const int all = (end + 63) >> 6;
   int p0, p1, slot = -1;
   if (a.own) {
@@ -686,7 +689,7 @@ __global__ void __launch_bounds__(64) chunk_merge_kernel(AttnArgs a) {
 }  // namespace k8s
 
 K8S_API int k8s_int8_attn_reply(const void* q, long ldq, const void* k, const void* v, const float* ks, const float* vs, int NB, const int* bt,
-                                int bt_stride, const int* ctx, const int* q_start, int S, int nq, int nkv, int BS, float scale, void* out,
+                                int bt_stride, int bt_cols, const int* ctx, const int* q_start, int S, int nq, int nkv, int BS, float scale, void* out,
                                 long ldo, float* part_o, float* part_ml, int n_parts, int part_size, const void* items, int n_items,
                                 const int* d_items, int grid, void* stream) {
   using namespace k8s::q8;
@@ -695,7 +698,7 @@ K8S_API int k8s_int8_attn_reply(const void* q, long ldq, const void* k, const vo
   if (n_parts > 1 && (!part_o || !part_ml || part_size <= 0 || (part_size & 63))) return (int)hipErrorInvalidValue;
   AttnArgs a{};
   a.q = (const uint16_t*)q, a.ldq = ldq, a.k = (const uint8_t*)k, a.v = (const uint8_t*)v, a.ks = ks, a.vs = vs, a.bt = bt;
-  a.bt_stride = bt_stride, a.NB = NB, a.ctx = ctx, a.q_start = q_start, a.S = S, a.nq = nq, a.nkv = nkv, a.G = nq / nkv, a.BS = BS;
+  a.bt_stride = bt_stride, a.bt_keys = (int)std::min((long)bt_cols * BS, 0x7fffffc0L), a.NB = NB, a.ctx = ctx, a.q_start = q_start, a.S = S, a.nq = nq, a.nkv = nkv, a.G = nq / nkv, a.BS = BS;
   a.scale_log2 = scale * kLog2e, a.out = (uint16_t*)out, a.ldo = ldo, a.part_o = part_o, a.part_ml = part_ml, a.n_parts = n_parts;
   a.part_size = part_size, a.items = (const int4*)items, a.n_items = n_items, a.d_items = d_items;
   hipStream_t st = (hipStream_t)stream;
@@ -707,7 +710,7 @@ K8S_API int k8s_int8_attn_reply(const void* q, long ldq, const void* k, const vo
 // Tiles of up to `rows` (token, q head) rows; split tiles leave parts of slot_rows rows a slot and kv head.  With own > 0 the lists are not
 // read: n_tiles is the most tiles of `own` tokens that the rows can make, and each one's keys are cut into `parts` runs.
 K8S_API int k8s_int8_attn_chunk(const void* q, long ldq, const void* k, const void* v, const float* ks, const float* vs, int NB, const int* bt,
-                                int bt_stride, const int* ctx, const int* q_start, int S, int nq, int nkv, int BS, float scale, void* out, long ldo,
+                                int bt_stride, int bt_cols, const int* ctx, const int* q_start, int S, int nq, int nkv, int BS, float scale, void* out, long ldo,
                                 const int* tile_seq, const int* tile_tok0, const int* tile_len, const int* tile_kv0, const int* tile_kv1,
                                 const int* tile_slot, int n_tiles, int rows, const int* m_tok0, const int* m_len, const int* m_slot0,
                                 const int* m_np, int n_merge, float* part_o, float* part_ml, int slot_rows, int own, int parts, void* stream) {
@@ -719,7 +722,7 @@ K8S_API int k8s_int8_attn_chunk(const void* q, long ldq, const void* k, const vo
   if (merged > 0 && (!part_o || !part_ml)) return (int)hipErrorInvalidValue;
   AttnArgs a{};
   a.q = (const uint16_t*)q, a.ldq = ldq, a.k = (const uint8_t*)k, a.v = (const uint8_t*)v, a.ks = ks, a.vs = vs, a.bt = bt;
-  a.bt_stride = bt_stride, a.NB = NB, a.ctx = ctx, a.q_start = q_start, a.S = S, a.nq = nq, a.nkv = nkv, a.G = nq / nkv, a.BS = BS;
+  a.bt_stride = bt_stride, a.bt_keys = (int)std::min((long)bt_cols * BS, 0x7fffffc0L), a.NB = NB, a.ctx = ctx, a.q_start = q_start, a.S = S, a.nq = nq, a.nkv = nkv, a.G = nq / nkv, a.BS = BS;
   a.scale_log2 = scale * kLog2e, a.out = (uint16_t*)out, a.ldo = ldo, a.part_o = part_o, a.part_ml = part_ml, a.own = own, a.parts = runs;
   a.tile_seq = tile_seq, a.tile_tok0 = tile_tok0, a.tile_len = tile_len, a.tile_kv0 = tile_kv0, a.tile_kv1 = tile_kv1, a.tile_slot = tile_slot;
   a.n_tiles = n_tiles, a.m_tok0 = m_tok0, a.m_len = m_len, a.m_slot0 = m_slot0, a.m_np = m_np;

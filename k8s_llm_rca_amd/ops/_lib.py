@@ -183,8 +183,8 @@ _SIGS = {
     "k8s_int8_gemm": [P, L, P, P, L, P, P, P, L, I, I, I, I, I, I, P, L, P],
     "k8s_int8_gemm_plan": [I, I, I],
     "k8s_int8_gemm_part": [I, I, I, I],
-    "k8s_int8_attn_reply": [P, L, P, P, P, P, I, P, I, P, P, I, I, I, I, F, P, L, P, P, I, I, P, I, P, I, P],
-    "k8s_int8_attn_chunk": [P, L, P, P, P, P, I, P, I, P, P, I, I, I, I, F, P, L, P, P, P, P, P, P, I, I, P, P, P, P, I, P, P, I, I, I, P],
+    "k8s_int8_attn_reply": [P, L, P, P, P, P, I, P, I, I, P, P, I, I, I, I, F, P, L, P, P, I, I, P, I, P, I, P],
+    "k8s_int8_attn_chunk": [P, L, P, P, P, P, I, P, I, I, P, P, I, I, I, I, F, P, L, P, P, P, P, P, P, I, I, P, P, P, P, I, P, P, I, I, I, P],
     "k8s_walks": [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, P, P, P, P],
 }
 # entry points whose C return type is not int

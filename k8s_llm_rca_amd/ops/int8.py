@@ -305,7 +305,8 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of ``q`` [T, >= nq 128] (row stride free) over the 8-bit pages -> [T, nq 128], for reply tokens and
     chunks alike.  ``meta`` is the step's, with the plan that ``attention.paged_attention`` takes (``attach_decode_plan`` or
-    ``attach_plan``): one plan serves both caches.  A row without a visible key gives zeros."""
+    ``attach_plan``): one plan serves both caches.  A row without a visible key gives zeros.  A context ends
+    where its row of the table does; a page that the pool does not have counts as its nearest one."""
     T = q.shape[0]
     _heads(q, cache, nq, nkv, nq * HEAD_DIM, "q")
     NB, _, BS, D = cache.k.shape
@@ -331,7 +332,7 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
         raise ValueError("q's rows must be dense and start at multiples of 16 bytes")
     G = nq // nkv
     common = (q.data_ptr(), ldq, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), NB,
-              bt.data_ptr(), bt.stride(0) if S > 1 else bt.shape[1], ctx.data_ptr(), starts.data_ptr())
+              bt.data_ptr(), bt.stride(0) if S > 1 else bt.shape[1], bt.shape[1], ctx.data_ptr(), starts.data_ptr())
     if meta.decode:
         if T != S:
             raise ValueError(f"a reply step has one row a sequence, not {T} for {S}")
@@ -422,13 +423,13 @@ def _attention_plain(q, cache: Int8KV, meta: A.AttnMeta, nq, nkv, scale, out):
     starts, ctx = meta.q_start.tolist(), meta.ctx_lens.tolist()
     BS, D, G = cache.k.shape[2], HEAD_DIM, nq // nkv
     for s in range(meta.num_seqs):
-        n, c = starts[s + 1] - starts[s], max(0, ctx[s])
-        at = meta.block_tables[s, :-(-c // BS)].long()
+        n, c = starts[s + 1] - starts[s], min(max(0, ctx[s]), meta.block_tables.shape[1] * BS)
+        at = meta.block_tables[s, :-(-c // BS)].long().clamp(0, cache.k.shape[0] - 1)
         k = (cache.k[at].float() * cache.k_scale[at][..., None]).permute(1, 0, 2, 3).reshape(nkv, -1, D)[:, :c]
         v = (cache.v[at].float() * cache.v_scale[at][:, :, None]).permute(1, 0, 3, 2).reshape(nkv, -1, D)[:, :c]
         rows = q[starts[s]:starts[s] + n, :nq * D].float().view(n, nkv, G, D).permute(1, 2, 0, 3)
         x = torch.matmul(rows, k[:, None].transpose(-1, -2)) * scale
-        hidden = torch.arange(c) > (c - n + torch.arange(n))[:, None]
+        hidden = torch.arange(c) > (ctx[s] - n + torch.arange(n))[:, None]
         x = x.masked_fill(hidden, -math.inf)
         p = torch.softmax(x, -1).masked_fill(hidden, 0.0)  # (a row without a key: zeros)
         o = torch.matmul(p, v[:, None]) if c else torch.zeros(nkv, G, n, D)

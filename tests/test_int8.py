@@ -841,6 +841,49 @@ def test_a_plan_for_fewer_query_heads_a_key_head_is_refused():
     check_attention(Q.paged_attention_int8(q, cache, meta, 16, 2, 0.09), q, cache, meta, starts, ctx, 16, 2, 0.09)
 
 
+def row_by_row(meta, starts, ctx, keys):
+    """The same rows as sequences of one row each, with the keys that each one sees of a table of `keys`."""
+    seq = [s for s in range(len(ctx)) for _ in range(starts[s], starts[s + 1])]
+    lens = [min(ctx[s] - (starts[s + 1] - starts[s]) + t - starts[s] + 1, keys) for t, s in enumerate(seq)]
+    one = A.AttnMeta(block_tables=meta.block_tables[seq], ctx_lens=None, q_start=None, num_seqs=len(seq), decode=True)
+    return one, list(range(len(seq) + 1)), lens
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lens,nq,nkv", [([(1, 700), (1, 300), (1, 640)], 8, 2), ([(70, 640), (3, 200), (64, 640)], 8, 2), ([(70, 640), (3, 200), (9, 630)], 10, 2)])
+@pytest.mark.parametrize("over", [0, 1, 5, 200])
+def test_a_context_ends_where_its_row_of_the_table_does(device, lens, nq, nkv, over):
+    """The table is a slice of columns of a wider one, whose other entries name pages too."""
+    q, cache, meta, starts, ctx = attn_case(device, lens, nq, nkv, NB=40)
+    bt = meta.block_tables[:, :10]
+    wide = torch.full((len(lens), 30), 39, dtype=torch.int32, device=device)
+    wide[:, 12:22] = bt
+    meta.block_tables = wide[:, 12:22]
+    cache.k_scale.copy_(torch.where(torch.isnan(cache.k_scale), 0.02, cache.k_scale))          # (every key is a number here)
+    cache.v_scale.copy_(torch.where(torch.isnan(cache.v_scale), 0.03, cache.v_scale))
+    ctx = [c + over if c >= 640 else c for c in ctx]
+    meta.ctx_lens = torch.tensor(ctx, dtype=torch.int32, device=device)
+    if device == "cuda":
+        planned(meta, starts, ctx, nq, nkv, 64)
+    out = Q.paged_attention_int8(q, cache, meta, nq, nkv, 0.09)
+    one, rows, seen = row_by_row(meta, starts, ctx, 640)
+    check_attention(out, q, cache, one, rows, seen, nq, nkv, 0.09)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lens,nq,nkv", [([(1, 700), (1, 300)], 8, 2), ([(70, 640), (3, 200)], 8, 2), ([(70, 640), (3, 200)], 10, 2)])
+def test_pages_that_the_pool_does_not_have_count_as_the_nearest(device, lens, nq, nkv):
+    q, cache, meta, starts, ctx = attn_case(device, lens, nq, nkv, NB=40)
+    for t in (cache.k_scale, cache.v_scale):
+        t.copy_(torch.where(torch.isnan(t), 0.02, t))
+    if device == "cuda":
+        planned(meta, starts, ctx, nq, nkv, 64)
+    meta.block_tables[0, 2], meta.block_tables[0, 5], meta.block_tables[1, 0] = 0, 39, 39
+    want = Q.paged_attention_int8(q, cache, meta, nq, nkv, 0.09)
+    meta.block_tables[0, 2], meta.block_tables[0, 5], meta.block_tables[1, 0] = -5, 40, 2 ** 31 - 1
+    assert torch.equal(Q.paged_attention_int8(q, cache, meta, nq, nkv, 0.09), want)
+
+
 # ------------------------------------------------------------------ refusals
 def test_refusals():
     x, w = torch.randn(4, 64), torch.ones(64)
