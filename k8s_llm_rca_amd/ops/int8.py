@@ -16,19 +16,23 @@ A layer in 8 bits, with weights from ``quantize_rows(w)``::
     x = linear_int8(*silu_mul_int8(linear_int8(y, ys, wgu, wgu_s)), wdown, wdown_s)
 
 Device tensors run on ``csrc/kernels/int8_*.hip``, on the current stream of their device; CPU tensors on the plain PyTorch
-forms below.  There are no gradients: under grad mode, inputs that ask for one are refused.
+forms below.  There are no gradients: under grad mode, inputs that ask for one are refused, and so are those with a forward-mode
+tangent.  On the device, calls inside ``torch.func`` transforms of their tensors and under ``torch.jit.trace`` or ``make_fx`` are
+refused too, which would not see the launch.
 """
 from __future__ import annotations
 
 import math
+import sys
 from dataclasses import dataclass
 from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import attention as A
-from ._lib import _raw_stream, check, lib, ptr, scratch
+from ._lib import _dispatch_modes, _raw_stream, _tracing, _transforms, check, lib, ptr, scratch
 
 HEAD_DIM = A.HEAD_DIM
 TINY = 2.0 ** -100
@@ -42,7 +46,7 @@ _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device
 
 
 def _inputs(*tensors) -> int:
-    """One device for all, whose number this is (-1: the CPU); none that asks for a gradient."""
+    """One device for all, whose number this is (-1: the CPU); none that asks for a gradient or that a launch by address would miss."""
     dev = tensors[0].get_device()
     for t in tensors:
         if t is not None and t.get_device() != dev:
@@ -51,7 +55,24 @@ def _inputs(*tensors) -> int:
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError(_NO_GRADIENT)
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(_NO_GRADIENT)
+    if dev >= 0 and (_tracing() is not None or _transforms() is not None or _dispatch_modes()):
+        _seen(tensors)
     return dev
+
+
+def _seen(tensors) -> None:
+    """Refuses what records or rewrites torch's operators: it would have no part in a kernel launched by address."""
+    if _tracing() is not None:
+        raise RuntimeError("the 8-bit operators cannot be traced on the device: a trace would not hold the launch")
+    if _transforms() is not None and any(torch._C._functorch.is_functorch_wrapped_tensor(t) for t in tensors if t is not None):
+        raise RuntimeError("the 8-bit operators take no part in torch.func transforms on the device")
+    fx = sys.modules.get("torch.fx.experimental.proxy_tensor")
+    if fx is not None and fx.get_proxy_mode() is not None:
+        raise RuntimeError("the 8-bit operators cannot be traced on the device: a trace would not hold the launch")
 
 
 def _call(name: str, dev: int, *args) -> None:
@@ -229,6 +250,8 @@ class Int8KV:
     v_scale: torch.Tensor
 
     def __post_init__(self):
+        if _transforms() is not None and self.k.get_device() >= 0:
+            _seen((self.k, self.v, self.k_scale, self.v_scale))
         NB, nkv, BS, D = self.k.shape
         if D != HEAD_DIM or self.v.shape != (NB, nkv, D, BS):
             raise ValueError("k must be [NB, nkv, BS, 128] and v [NB, nkv, 128, BS]")
@@ -268,7 +291,7 @@ def rope_kv_write_int8(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torc
     takes its nearest row.  As in ``attention.rope_kv_write``, the rows of one call have different slots."""
     T = qkv.shape[0]
     _heads(qkv, cache, nq, nkv, (nq + 2 * nkv) * HEAD_DIM, "qkv")
-    dev = _inputs(qkv, positions, cos_sin, slots, cache.k)
+    dev = _inputs(qkv, positions, cos_sin, slots, cache.k_scale, cache.v_scale)
     for t in (positions, slots):
         if t is not None and (t.dtype != torch.int32 or t.shape != (T,) or not t.is_contiguous()):
             raise ValueError(f"positions and slots must be contiguous int32 {[T]}, not {t.dtype} {list(t.shape)}")
@@ -311,7 +334,7 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
     _heads(q, cache, nq, nkv, nq * HEAD_DIM, "q")
     NB, _, BS, D = cache.k.shape
     S, bt, ctx, starts = meta.num_seqs, meta.block_tables, meta.ctx_lens, meta.q_start
-    dev = _inputs(q, bt, ctx, starts, cache.k, out)
+    dev = _inputs(q, bt, ctx, starts, cache.k_scale, cache.v_scale, out)
     if out is None:
         out, ldo = torch.empty((T, nq * D), dtype=q.dtype, device=q.device), nq * D
     else:
@@ -326,6 +349,8 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
         raise ValueError("block_tables must be int32 [S, pages]")
     if S > 1 and bt.stride(0) < bt.shape[1]:
         raise ValueError("the rows of block_tables overlap")
+    if _transforms() is not None:
+        _seen(t for t in vars(meta).values() if isinstance(t, torch.Tensor))
     ctx, starts = _lengths(ctx, starts, S)
     ldq = _pitch(q)
     if not ldq:

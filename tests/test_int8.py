@@ -993,6 +993,70 @@ def test_refusals_of_plans_and_tables(lens, nq):
         Q.paged_attention_int8(q, cache, meta, nq, 2, 1.0)
 
 
+def calls(device):
+    """Each operator as a function of one of its floating-point inputs, and that input."""
+    g = gen(8)
+    x, w = randn(g, 4, 64, device=device), randn(g, 64, device=device)
+    q, s = Q.quantize_rows(x)
+    qkv, pos, at = (t.to(device) for t in write_case(3, 4, 2, 64, [1, 2, 3]))
+    cs = table(512).to(device)
+    cache = noise(Q.Int8KV.empty(4, 2, 64, device))
+    rows, _, meta, starts, ctx = attn_case(device, [(1, 70), (1, 3)], 4, 2)
+    if device == "cuda":
+        planned(meta, starts, ctx, 4, 2, 64)
+    held = lambda f: lambda t: Q.Int8KV(cache.k, cache.v, *f(t))  # noqa: E731
+    ks, vs = held(lambda t: (t, cache.v_scale)), held(lambda t: (cache.k_scale, t))
+    return [(lambda t: Q.quantize_rows(t)[1], x), (lambda t: Q.silu_mul_int8(t)[1], x), (lambda t: Q.rmsnorm_int8(t, w, 1e-5)[1], x),
+            (lambda t: Q.rmsnorm_int8(x, t, 1e-5)[1], w), (lambda t: Q.rmsnorm_int8(x, w, 1e-5, residual=t)[1], x.clone()),
+            (lambda t: Q.linear_int8(q, t, q, s), s), (lambda t: Q.linear_int8(q, s, q, t), s), (lambda t: Q.linear_int8(q, s, q, s, bias=t), s),
+            (lambda t: Q.rope_kv_write_int8(t, pos, cs, at, cache, 4, 2), qkv), (lambda t: Q.rope_kv_write_int8(qkv, pos, t, at, cache, 4, 2), cs),
+            (lambda t: Q.rope_kv_write_int8(qkv, pos, cs, at, ks(t), 4, 2), cache.k_scale),
+            (lambda t: Q.paged_attention_int8(t, cache, meta, 4, 2, 1.0), rows), (lambda t: Q.paged_attention_int8(rows, ks(t), meta, 4, 2, 1.0), cache.k_scale),
+            (lambda t: Q.paged_attention_int8(rows, vs(t), meta, 4, 2, 1.0), cache.v_scale)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_no_derivative_in_either_direction(device):
+    for f, t in calls(device):
+        leaf = t.clone().requires_grad_(True)
+        with pytest.raises(RuntimeError, match="no gradients"):
+            f(leaf)
+        with torch.no_grad():
+            f(leaf.detach())
+        with torch.autograd.forward_ad.dual_level():
+            f(t.clone())
+            with pytest.raises(RuntimeError, match="no gradients"):
+                f(torch.autograd.forward_ad.make_dual(t.clone(), torch.ones_like(t)))
+
+
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore")
+def test_what_records_calls_is_refused_on_the_device():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for f, t in calls("cuda"):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(f, t.clone(), check_trace=False)
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(f)(t.clone())
+        with pytest.raises(RuntimeError, match="torch.func"):
+            torch.func.functionalize(f)(t.clone())
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(f)(t.clone()[None])
+        f(t.clone())
+        torch.func.vmap(lambda z: (f(t.clone()), z)[1])(torch.zeros(2, device="cuda"))       # (its own tensors are not the transform's)
+        with torch.device("cuda"):
+            f(t.clone())
+    q, cache, meta, starts, ctx = attn_case("cuda", [(1, 70), (1, 3)], 4, 2)
+    planned(meta, starts, ctx, 4, 2, 64)
+
+    def with_items(t):
+        meta.items = t
+        return Q.paged_attention_int8(q, cache, meta, 4, 2, 1.0)
+
+    with pytest.raises(RuntimeError, match="torch.func"):
+        torch.func.functionalize(with_items)(meta.items.clone())
+
+
 # ------------------------------------------------------------------ together
 class Layer:
     """A decoder layer in 8 bits, as the module's docstring has it."""
