@@ -10,8 +10,9 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// Below this a row's largest value is stored as zero: its reciprocal times 127 would come near fp32's end.
-constexpr float kTiny = 0x1p-100f;
+// Below this a row's largest value is stored as zero.  Behind a norm that goes by y, and the h w that the integers are made of go
+// down to kLeast, whose reciprocal times 127 is near fp32's end (with eps of 2^-40 and more y is below kTiny before that).
+constexpr float kTiny = 0x1p-100f, kLeast = 0x1p-120f;
 
 // max|y| as bits: a NaN is larger than the infinity, so that neither is lost on the way
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
@@ -20,10 +21,10 @@ struct Step {
   float inv, rest;  // integers a unit of y, and what rounding it left
   float scale;      // what an integer stands for; NaN where the row holds a NaN or an infinity (its integers are zeros)
 };
-__device__ __forceinline__ Step row_step(uint32_t top) {
+__device__ __forceinline__ Step row_step(uint32_t top, float least = kTiny) {
   const float t = __uint_as_float(top);
   if (top >= 0x7f800000u) return {0.f, 0.f, __uint_as_float(0x7fc00000u)};
-  if (t < kTiny) return {0.f, 0.f, 0.f};
+  if (t < least) return {0.f, 0.f, 0.f};
   const float inv = 127.f / t;
   return {inv, fmaf(-inv, t, 127.f) / t, t / 127.f};
 }

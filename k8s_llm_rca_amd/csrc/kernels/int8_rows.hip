@@ -141,13 +141,14 @@ __global__ void __launch_bounds__(W >= 4 ? 64 * W : 256) rows_kernel(RowArgs a) 
       ss += sums[k];
     }
   }
-  const Step s = row_step(top);
+  Step s = row_step(top, MODE == NORM ? kLeast : kTiny);
   uint8_t* const q = a.q + (size_t)row * a.ldq;
-  if (t == 0) {
-    float sc = s.scale;
-    if constexpr (MODE == NORM) sc *= 1.f / sqrtf(ss / (float)a.H + a.eps);
-    a.scale[row] = sc;
+  if constexpr (MODE == NORM) {
+    const float f = 1.f / sqrtf(ss / (float)a.H + a.eps);
+    s.scale *= f;
+    if (__uint_as_float(top) * f < kTiny) s = {0.f, 0.f, 0.f};
   }
+  if (t == 0) a.scale[row] = s.scale;
   if constexpr (NC > 0) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {

@@ -3,7 +3,9 @@
 A row ``y`` stands as integers ``q = round(127 y / max|y|)`` (ties to even) and the scale ``max|y| / 127``: one scale for each
 row of an activation, each output channel of a weight, each token and head of a cached key or value.  A row whose largest
 value is below 2^-100 is stored as zeros with the scale 0; one that holds a NaN or an infinity as zeros with the scale NaN,
-so that what is computed from it is NaN and not a number that looks like one.
+so that what is computed from it is NaN and not a number that looks like one.  Behind a norm the row is that of the whole formula;
+its products of values and weights, in front of the norm's factor, are fp32's: those past its end count as infinities, and a
+row of products below 2^-120 as zeros.
 
 A layer in 8 bits, with weights from ``quantize_rows(w)``::
 
@@ -35,7 +37,7 @@ from . import attention as A
 from ._lib import _dispatch_modes, _raw_stream, _tracing, _transforms, check, lib, ptr, scratch
 
 HEAD_DIM = A.HEAD_DIM
-TINY = 2.0 ** -100
+TINY, LEAST = 2.0 ** -100, 2.0 ** -120
 #: K of a product, at most: the sum of K products of 128 x 128 stays below 2^31
 MAX_K = 131056
 _ROW_TYPES = (torch.bfloat16, torch.float32)
@@ -150,7 +152,9 @@ def _rows(mode: int, x: torch.Tensor, H: int, out, scale, w=None, residual=None,
         if residual is not None:
             residual.copy_(y + residual.float())
             y = residual.float()
+        top = (y * w.float()).abs().amax(-1, keepdim=True)
         y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + eps) * w.float()
+        y = y.masked_fill(top < LEAST, 0.0).masked_fill(~torch.isfinite(top), math.nan)
     q, s = _quantised(y)
     out.copy_(q)
     scale.copy_(s)

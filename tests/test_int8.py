@@ -119,6 +119,35 @@ def test_rows_that_hold_no_number(device, H):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T,H", [(4, 64), (4, 4096), (4, 16400), (4, 33008), (1500, 2064)])
+def test_a_norm_s_row_is_zero_by_what_the_norm_gives(device, dtype, T, H):
+    """Values below 2^-100 in front of the norm's factor and above it behind, and the other way round; products that leave fp32."""
+    g = gen(H)
+    x = (1 + torch.rand(T, H, generator=g)) * torch.where(torch.rand(T, H, generator=g) < 0.5, -1.0, 1.0)
+    one = torch.ones(H, dtype=dtype)
+
+    def both(x, w, eps):
+        x = x.to(dtype)
+        h = x.double()
+        q, s = Q.rmsnorm_int8(x.to(device), w.to(device), eps)
+        check_rows(q, s, h * w.double() / (h.square().mean(-1, keepdim=True) + eps).sqrt(), 2.0 ** -22, 2.0 ** -17)
+        return q, s
+
+    q, s = both(x * 2.0 ** -103, one, 1e-5)                    # y = 2^-94 and more
+    assert q.any(1).all() and (s > 0).all()
+    q, s = both(x * 2.0 ** -110, one, 1e-5)                    # y = 2^-100.7 at most
+    q, s = both(x * 2.0 ** -115, one, 1e-12)                   # y = 2^-95
+    assert q.any(1).all()
+    q, s = both(4 * x, one * 2.0 ** -101, 1e-5)                # h w = 2^-98, y = 2^-100.5 at most
+    assert not q.any() and not s.any()
+    q, s = Q.rmsnorm_int8((x * 2.0 ** -122).to(dtype).to(device), one.to(device), 1e-14)      # (y = 2^-98, of h w below 2^-120)
+    assert not q.any() and not s.any()
+    q, s = Q.rmsnorm_int8((x * 2.0 ** 40).to(dtype).to(device), (one * 2.0 ** 100).to(device), 1e-5)
+    assert not q.any() and torch.isnan(s).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_ties_go_to_even(device):
     """Rows of short numbers, every one of which may lie half way between two integers: the integers of the definition, exactly."""
     top = torch.arange(128, 256, dtype=F64)                   # every bf16 mantissa as the row's maximum
