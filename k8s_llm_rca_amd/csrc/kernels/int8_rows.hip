@@ -147,6 +147,7 @@ __global__ void __launch_bounds__(W >= 4 ? 64 * W : 256) rows_kernel(RowArgs a) 
     const float f = 1.f / sqrtf(ss / (float)a.H + a.eps);
     s.scale *= f;
     if (__uint_as_float(top) * f < kTiny) s = {0.f, 0.f, 0.f};
+    if (!(ss < INFINITY)) s = {0.f, 0.f, __uint_as_float(0x7fc00000u)};  // (squares that left fp32: no zeros for them)
   }
   if (t == 0) a.scale[row] = s.scale;
   if constexpr (NC > 0) {

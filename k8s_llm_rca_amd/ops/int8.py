@@ -4,8 +4,8 @@ A row ``y`` stands as integers ``q = round(127 y / max|y|)`` (ties to even) and 
 row of an activation, each output channel of a weight, each token and head of a cached key or value.  A row whose largest
 value is below 2^-100 is stored as zeros with the scale 0; one that holds a NaN or an infinity as zeros with the scale NaN,
 so that what is computed from it is NaN and not a number that looks like one.  Behind a norm the row is that of the whole formula;
-its products of values and weights, in front of the norm's factor, are fp32's: those past its end count as infinities, and a
-row of products below 2^-120 as zeros.
+its products of values and weights, in front of the norm's factor, and its sum of squares are fp32's: past its end they count as
+infinities, and a row of products below 2^-120 as zeros.
 
 A layer in 8 bits, with weights from ``quantize_rows(w)``::
 
@@ -153,8 +153,9 @@ def _rows(mode: int, x: torch.Tensor, H: int, out, scale, w=None, residual=None,
             residual.copy_(y + residual.float())
             y = residual.float()
         top = (y * w.float()).abs().amax(-1, keepdim=True)
-        y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + eps) * w.float()
-        y = y.masked_fill(top < LEAST, 0.0).masked_fill(~torch.isfinite(top), math.nan)
+        ss = y.square().mean(-1, keepdim=True)
+        y = y * torch.rsqrt(ss + eps) * w.float()
+        y = y.masked_fill(top < LEAST, 0.0).masked_fill(~(torch.isfinite(top) & torch.isfinite(ss)), math.nan)
     q, s = _quantised(y)
     out.copy_(q)
     scale.copy_(s)

@@ -148,6 +148,24 @@ def test_a_norm_s_row_is_zero_by_what_the_norm_gives(device, dtype, T, H):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("H", [64, 4096, 16400, 33008])
+def test_squares_that_leave_fp32_give_no_zeros(device, dtype, H):
+    """Values of 2^54 are normed as any, values of 2^66 leave nothing to norm them by."""
+    x = (1 + torch.rand(4, H, generator=gen(H))).to(dtype)
+    x[:2] *= 2.0 ** 66
+    x[2:] *= 2.0 ** 54
+    w = torch.ones(H, dtype=dtype)
+    r = torch.zeros_like(x).to(device)
+    for residual in (None, r):
+        q, s = Q.rmsnorm_int8(x.to(device), w.to(device), 1e-5, residual=residual)
+        assert torch.isnan(s[:2]).all() and not q[:2].any()
+        h = x[2:].double()
+        check_rows(q[2:], s[2:], h / h.square().mean(-1, keepdim=True).sqrt(), 2.0 ** -22, 2.0 ** -17)
+    assert torch.equal(r.cpu(), x)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_ties_go_to_even(device):
     """Rows of short numbers, every one of which may lie half way between two integers: the integers of the definition, exactly."""
     top = torch.arange(128, 256, dtype=F64)                   # every bf16 mantissa as the row's maximum
