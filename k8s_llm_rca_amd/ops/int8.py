@@ -101,6 +101,11 @@ def _pitch(t: torch.Tensor) -> int:
     return 0 if ld * t.element_size() & 15 else ld
 
 
+def _apart(t: torch.Tensor) -> bool:
+    """Whether the rows of a matrix that is written lie apart."""
+    return t.shape[0] <= 1 or t.stride(0) >= t.shape[1]
+
+
 def _quantised(y: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """The plain form on the last axis of an fp32 tensor (the quotient in 64 bits, so that ties are ties)."""
     top = y.abs().amax(-1, keepdim=True)
@@ -122,9 +127,9 @@ def _rows(mode: int, x: torch.Tensor, H: int, out, scale, w=None, residual=None,
     if out is None:
         out, ldq = torch.empty((T, H), dtype=torch.int8, device=x.device), H
     else:
-        ldq = _pitch(out) if out.dtype == torch.int8 and out.shape == (T, H) else 0
+        ldq = _pitch(out) if out.dtype == torch.int8 and out.shape == (T, H) and _apart(out) else 0
         if not ldq:
-            raise ValueError(f"out must be int8 {[T, H]} with 16-byte rows")
+            raise ValueError(f"out must be int8 {[T, H]} with 16-byte rows that lie apart")
     if scale is None:
         scale = torch.empty(T, dtype=torch.float32, device=x.device)
     elif scale.dtype != torch.float32 or scale.shape != (T,) or not scale.is_contiguous():
@@ -220,8 +225,8 @@ def linear_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
             raise TypeError(f"out_dtype must be bfloat16 or float32, not {out_dtype}")
         out, ldy = torch.empty((M, N), dtype=out_dtype, device=x.device), N
     else:
-        if out.dtype not in _ROW_TYPES or out.shape != (M, N) or (out.stride(1) != 1 and N > 1):
-            raise ValueError(f"out must be bfloat16 or float32 {[M, N]}, its rows dense")
+        if out.dtype not in _ROW_TYPES or out.shape != (M, N) or (out.stride(1) != 1 and N > 1) or not _apart(out):
+            raise ValueError(f"out must be bfloat16 or float32 {[M, N]}, its rows dense and apart")
         ldy = out.stride(0) if M > 1 else N
     if M == 0 or N == 0:
         return out
@@ -302,6 +307,8 @@ def rope_kv_write_int8(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torc
             raise ValueError(f"positions and slots must be contiguous int32 {[T]}, not {t.dtype} {list(t.shape)}")
     if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or cos_sin.dim() != 2 or cos_sin.shape[1] != HEAD_DIM or not cos_sin.shape[0]:
         raise ValueError("cos_sin must be contiguous float32 [positions, 128]")
+    if not _apart(qkv):
+        raise ValueError("the rows of qkv, which are written, must lie apart")
     NB, _, BS, D = cache.k.shape
     if T == 0:
         return
@@ -343,8 +350,8 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
     if out is None:
         out, ldo = torch.empty((T, nq * D), dtype=q.dtype, device=q.device), nq * D
     else:
-        if out.shape != (T, nq * D) or out.dtype != q.dtype or out.stride(1) != 1:
-            raise ValueError("out must be [T, nq 128] of q's type, its rows dense")
+        if out.shape != (T, nq * D) or out.dtype != q.dtype or out.stride(1) != 1 or not _apart(out):
+            raise ValueError("out must be [T, nq 128] of q's type, its rows dense and apart")
         ldo = out.stride(0) if T > 1 else nq * D
     if T == 0 or S == 0:
         return out

@@ -1010,6 +1010,30 @@ def test_refusals_of_the_cache():
         Q.paged_attention_int8(q, cache, meta, 4, 2, 1.0, out=torch.empty(2, 512))
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_rows_that_are_written_lie_apart(device):
+    """Rows that share memory, in steps that every other check lets pass."""
+    x = randn(gen(1), 4, 64, device=device)
+    shared = lambda rows, width, step, dtype: torch.zeros(rows * width, dtype=dtype, device=device).as_strided((rows, width), (step, 1))  # noqa: E731
+    with pytest.raises(ValueError):
+        Q.quantize_rows(x, out=shared(4, 64, 48, torch.int8))
+    q, s = Q.quantize_rows(x, out=shared(4, 64, 64, torch.int8))
+    for step in (0, 2):
+        with pytest.raises(ValueError):
+            Q.linear_int8(q, s, q, s, out=shared(4, 4, step, F32))
+    Q.linear_int8(q[:1], s[:1], q, s, out=shared(1, 4, 0, F32))
+    qkv, pos, at = (t.to(device) for t in write_case(3, 4, 2, 64, [1, 2, 3]))
+    cache = Q.Int8KV.empty(4, 2, 64, device)
+    with pytest.raises(ValueError):
+        Q.rope_kv_write_int8(shared(3, 8 * D, 7 * D, BF), pos, table(512).to(device), at, cache, 4, 2)
+    rows, cache, meta, starts, ctx = attn_case(device, [(1, 70), (1, 3)], 4, 2)
+    if device == "cuda":
+        planned(meta, starts, ctx, 4, 2, 64)
+    with pytest.raises(ValueError):
+        Q.paged_attention_int8(rows, cache, meta, 4, 2, 1.0, out=shared(2, 4 * D, 3 * D, BF))
+    Q.paged_attention_int8(rows, cache, meta, 4, 2, 1.0, out=shared(2, 4 * D, 4 * D, BF))
+
+
 @pytest.mark.gpu
 def test_refusals_on_the_device():
     q, cache, meta, starts, ctx = attn_case("cuda", [(1, 70), (1, 3)], 4, 2)
