@@ -433,9 +433,9 @@ __global__ void __launch_bounds__(512, 1) chunk_kernel(AttnArgs a) {
     *reinterpret_cast<bf16x8*>(kr + 16 * ((2 * kc + 1) ^ (key & 15))) = to_bf16x8(kx[2], kx[3]);
     // a key behind the context is nothing, whatever its scales say; a value that is no number makes its key's score none, so
     // that the weights' factor is always a number (and a hidden key's product zero).  All waves write the same.
-    const bool in = 64 * (p0 + i) + lane < end, nan = vsx != vsx;
-    sm.p.s[i & 3][0][lane] = in ? (nan ? vsx : ksx * a.scale_log2) : 0.f;
-    sm.p.s[i & 3][1][lane] = in && !nan ? vsx : 0.f;
+    const bool in = 64 * (p0 + i) + lane < end, number = fabsf(vsx) < INFINITY;
+    sm.p.s[i & 3][0][lane] = in ? (number ? ksx * a.scale_log2 : __uint_as_float(0x7fc00000u)) : 0.f;
+    sm.p.s[i & 3][1][lane] = in && number ? vsx : 0.f;
   };
   auto keep_v = [&](int slot) {
     uint8_t* const vr = sm.p.v[slot] + dim * 128;

@@ -464,10 +464,13 @@ def _attention_plain(q, cache: Int8KV, meta: A.AttnMeta, nq, nkv, scale, out):
         at = meta.block_tables[s, :-(-c // BS)].long().clamp(0, cache.k.shape[0] - 1)
         k = (cache.k[at].float() * cache.k_scale[at][..., None]).permute(1, 0, 2, 3).reshape(nkv, -1, D)[:, :c]
         v = (cache.v[at].float() * cache.v_scale[at][:, :, None]).permute(1, 0, 3, 2).reshape(nkv, -1, D)[:, :c]
+        # a value's scale that is no number makes its key's score none, so that rows that do not see the key stay as they are
+        odd = ~torch.isfinite(cache.v_scale[at].permute(1, 0, 2).reshape(nkv, 1, 1, -1)[..., :c])
+        v = v.masked_fill(odd[:, 0, 0, :, None], 0.0)
         rows = q[starts[s]:starts[s] + n, :nq * D].float().view(n, nkv, G, D).permute(1, 2, 0, 3)
         x = torch.matmul(rows, k[:, None].transpose(-1, -2)) * scale
         hidden = torch.arange(c) > (ctx[s] - n + torch.arange(n))[:, None]
-        x = x.masked_fill(hidden, -math.inf)
+        x = x.masked_fill(odd, math.nan).masked_fill(hidden, -math.inf)
         p = torch.softmax(x, -1).masked_fill(hidden, 0.0)  # (a row without a key: zeros)
         o = torch.matmul(p, v[:, None]) if c else torch.zeros(nkv, G, n, D)
         out[starts[s]:starts[s] + n] = o.permute(2, 0, 1, 3).reshape(n, nq * D).to(out.dtype)

@@ -718,6 +718,26 @@ def test_a_key_without_a_number_reaches_the_rows_that_see_it(lens):
     assert torch.equal(out[:n][~sees], clean[:n][~sees]) and torch.equal(out[:, :2 * D], clean[:, :2 * D]) and torch.equal(out[n:], clean[n:])
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lens,nq", [([(1, 300), (1, 300)], 4), ([(40, 300), (40, 300)], 4), ([(40, 300), (40, 300)], 10), ([(6, 100)], 4)])
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+def test_a_scale_without_a_number_reaches_the_rows_that_see_it(device, lens, nq, which, what):
+    """One key of the last page; a row in front of it has the same bits as without it, a row behind it no number (but that a key's
+    infinite scale may stand for a score of -infinity)."""
+    q, cache, meta, starts, ctx = attn_case(device, lens, nq, 2)
+    if device == "cuda":
+        planned(meta, starts, ctx, nq, 2, 64)
+    clean = Q.paged_attention_int8(q, cache, meta, nq, 2, 0.09).clone()
+    n, c = lens[0]
+    getattr(cache, which)[meta.block_tables[0, (c - 4) // 64].long(), 1, (c - 4) % 64] = what
+    out = Q.paged_attention_int8(q, cache, meta, nq, 2, 0.09)
+    sees = torch.arange(n, device=device) + c - n >= c - 4
+    half = nq // 2 * D
+    assert bool(sees.any()) and (which == "k_scale" and math.isinf(what) or not bool(torch.isfinite(out[:n][sees][:, half:]).all(1).any()))
+    assert torch.equal(out[:n][~sees], clean[:n][~sees]) and torch.equal(out[:, :half], clean[:, :half]) and torch.equal(out[n:], clean[n:])
+
+
 @pytest.mark.gpu
 def test_pages_behind_two_gigabytes():
     NB = 34000                                               # 8 heads x 64 x 128: 2.2 GB of keys
