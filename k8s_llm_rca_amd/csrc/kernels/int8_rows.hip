@@ -194,14 +194,18 @@ K8S_API int k8s_int8_rows(int mode, int f32, const void* x, long ldx, void* res,
   using namespace k8s::q8;
   if (T <= 0) return 0;
   if (mode < 0 || mode > 2 || H <= 0 || (H & 7) || (mode == NORM && !w)) return (int)hipErrorInvalidValue;
-  const RowArgs a{x, res, w, (uint8_t*)q, scale, T, H, ldx, ldq, eps};
   hipStream_t st = (hipStream_t)stream;
-  switch (mode * 2 + (f32 ? 1 : 0)) {
-    case 0: return launch<ROWS, uint16_t>(a, st);
-    case 1: return launch<ROWS, float>(a, st);
-    case 2: return launch<GATE, uint16_t>(a, st);
-    case 3: return launch<GATE, float>(a, st);
-    case 4: return launch<NORM, uint16_t>(a, st);
-    default: return launch<NORM, float>(a, st);
+  const long size = f32 ? 4 : 2;
+  constexpr int kMost = 1 << 21;  // rows a launch: 2^31 threads (a grid holds fewer than 2^32)
+  for (int t0 = 0; t0 < T;) {
+    const int n = T - t0 < kMost ? T - t0 : kMost;
+    const RowArgs a{(const char*)x + t0 * ldx * size, res ? (char*)res + (long)t0 * H * size : nullptr, w, (uint8_t*)q + t0 * ldq, scale + t0, n, H, ldx,
+                    ldq, eps};
+    const int rc = mode == ROWS ? (f32 ? launch<ROWS, float>(a, st) : launch<ROWS, uint16_t>(a, st))
+                   : mode == GATE ? (f32 ? launch<GATE, float>(a, st) : launch<GATE, uint16_t>(a, st))
+                                  : (f32 ? launch<NORM, float>(a, st) : launch<NORM, uint16_t>(a, st));
+    if (rc) return rc;
+    t0 += n;
   }
+  return 0;
 }

@@ -91,6 +91,12 @@ def _stream(dev: int) -> int:
     return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
 
 
+def _countable(*counts: int) -> None:
+    """The kernels count rows and columns in 32 bits."""
+    if max(counts) >= 1 << 31:
+        raise ValueError(f"{max(counts)} rows or columns: at most 2^31 - 1 in one call")
+
+
 def _pitch(t: torch.Tensor) -> int:
     """Values from row to row of a matrix whose rows are dense and start at multiples of 16 bytes; 0 of another."""
     (n, width), (ld, one) = t.shape, t.stride()
@@ -140,6 +146,7 @@ def _rows(mode: int, x: torch.Tensor, H: int, out, scale, w=None, residual=None,
                                  or residual.data_ptr() & 15):
         raise ValueError("the residual must be contiguous, 16-byte aligned and of the rows' shape and type")
     if dev >= 0:
+        _countable(T)
         ld = _pitch(x)
         if not ld:
             x = x.clone(memory_format=torch.contiguous_format)
@@ -231,6 +238,7 @@ def linear_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
     if M == 0 or N == 0:
         return out
     if dev >= 0:
+        _countable(M, N)
         ldx, ldw = _pitch(x), _pitch(w)
         if not ldx:
             x = x.clone(memory_format=torch.contiguous_format)

@@ -106,6 +106,22 @@ def test_many_rows(T, H):
     check_rows(q, s, h * w.double() / (h.square().mean(-1, keepdim=True) + 1e-5).sqrt(), 2.0 ** -22, 2.0 ** -17)
 
 
+@pytest.mark.gpu
+def test_more_rows_than_one_grid_holds():
+    """70 million rows of 16: four rows a workgroup of 256 would be more than 2^32 threads."""
+    T = 70_000_003
+    x = torch.arange(T, device="cuda", dtype=torch.int32)[:, None].remainder(torch.arange(3, 19, device="cuda", dtype=torch.int32)).to(BF)
+    q, s = Q.quantize_rows(x)
+    for a, b in ((0, 1000), (2 ** 21 - 500, 2 ** 21 + 500), (2 ** 26 - 500, 2 ** 26 + 500), (T - 1000, T)):
+        check_rows(q[a:b], s[a:b], x[a:b], 2.0 ** -24)
+    r = torch.ones_like(x)
+    q, s = Q.rmsnorm_int8(x, torch.ones(16, dtype=BF, device="cuda"), 1e-5, residual=r)
+    assert torch.equal(r, x + 1)
+    for a, b in ((0, 1000), (2 ** 21 - 500, 2 ** 21 + 500), (2 ** 26 - 500, 2 ** 26 + 500), (T - 1000, T)):
+        h = r[a:b].double()
+        check_rows(q[a:b], s[a:b], h / (h.square().mean(-1, keepdim=True) + 1e-5).sqrt(), 2.0 ** -22, 2.0 ** -17)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("H", [128, 4096, 16384, 33008])
 def test_rows_that_hold_no_number(device, H):
@@ -1052,6 +1068,13 @@ def test_rows_that_are_written_lie_apart(device):
     with pytest.raises(ValueError):
         Q.paged_attention_int8(rows, cache, meta, 4, 2, 1.0, out=shared(2, 4 * D, 3 * D, BF))
     Q.paged_attention_int8(rows, cache, meta, 4, 2, 1.0, out=shared(2, 4 * D, 4 * D, BF))
+
+
+def test_counts_that_32_bits_do_not_hold_are_refused():
+    Q._countable(0, 2 ** 31 - 1)
+    for n in ((2 ** 31,), (3, 2 ** 32 + 1), (2 ** 40, 1)):
+        with pytest.raises(ValueError):
+            Q._countable(*n)
 
 
 @pytest.mark.gpu
