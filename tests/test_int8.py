@@ -284,6 +284,20 @@ def test_tiles_of_128_by_256(M, N, K, runs, monkeypatch):
         check_product(Q.linear_int8(*args[:4], bias=args[4], out_dtype=dtype), *args)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 6, 7, 13, 16])
+@pytest.mark.parametrize("N,K", [(1, 16), (33, 80), (515, 2064), (64, 4112), (47, Q.MAX_K)])
+def test_few_rows(M, N, K, monkeypatch):
+    """The kernel of up to 16 rows, whichever the plan would choose: no and several turns over K, a last one that is not whole."""
+    forced(monkeypatch, Q.FEW, 1)
+    for dtype in (BF, F32):
+        args = product_case("cuda", M, N, K, dtype, True)
+        check_product(Q.linear_int8(*args[:4], bias=args[4], out_dtype=dtype), *args)
+        big = torch.full((M, N + 5), 7.0, dtype=dtype, device="cuda")
+        check_product(Q.linear_int8(*args[:4], out=big[:, 3:N + 3]), *args[:4], None)
+        assert bool((big[:, :3] == 7).all() and (big[:, N + 3:] == 7).all())
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 1, 16), (3, 5, 48), (33, 17, 4096)])
 def test_product_plain(M, N, K):
     for dtype, bias in ((BF, False), (F32, True)):
@@ -466,6 +480,22 @@ def test_write_without_slots_and_without_rows(device):
     Q.rope_kv_write_int8(two, pos.to(device), cs, torch.arange(3, dtype=torch.int32, device=device), cache, 4, 2)
     assert torch.equal(one, two) and not torch.equal(one.cpu()[:, :512], qkv[:, :512])
     Q.rope_kv_write_int8(one[:0], pos.to(device)[:0], cs, None, cache, 4, 2)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T,nq,nkv", [(6, 4, 2), (700, 4, 8)])
+def test_positions_outside_the_table_take_its_nearest_row(device, T, nq, nkv):
+    qkv, _, at = write_case(T, nq, nkv, 64, range(T))
+    cs = table(40).to(device)
+    far = torch.randint(-60, 100, (T,), generator=gen(T), dtype=torch.int32)
+    far[:6] = torch.tensor([-1, 40, 39, 0, -2 ** 31, 2 ** 31 - 1], dtype=torch.int32)
+    got = []
+    for pos in (far, far.clamp(0, 39)):
+        cache = Q.Int8KV.empty(-(-T // 64), nkv, 64, device)
+        mine = qkv.clone().to(device)
+        Q.rope_kv_write_int8(mine, pos.to(device), cs, at.to(device), cache, nq, nkv)
+        got.append([mine, cache.k, cache.v, cache.k_scale, cache.v_scale])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
 
 
 @pytest.mark.parametrize("device", DEVICES)
