@@ -483,7 +483,7 @@ def test_write_without_slots_and_without_rows(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
-@pytest.mark.parametrize("T,nq,nkv", [(6, 4, 2), (700, 4, 8)])
+@pytest.mark.parametrize("T,nq,nkv", [(6, 4, 2), (700, 8, 8)])
 def test_positions_outside_the_table_take_its_nearest_row(device, T, nq, nkv):
     qkv, _, at = write_case(T, nq, nkv, 64, range(T))
     cs = table(40).to(device)
