@@ -21,6 +21,9 @@ namespace q8 {
 constexpr int D = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 
+struct Item {  // (a list may begin at any word of a step's buffer)
+  int x, y, z, w;
+};
 struct AttnArgs {
   const uint16_t* q;
   long ldq;
@@ -35,7 +38,7 @@ struct AttnArgs {
   uint16_t* out;
   long ldo;
   // replies: a list of (row, part | -1, end key, q row | (tokens - 1) << 24), parts of part_size keys
-  const int4* items;
+  const Item* items;
   int n_items;
   const int* d_items;  // {items, keys a part} on the device, of n_items that the list has room for; or null
   float *part_o, *part_ml;
@@ -213,7 +216,7 @@ __global__ void __launch_bounds__(64, 2) reply_kernel(AttnArgs a) {
   const int total = n_items * a.nkv;
   for (int w = blockIdx.x; w < total; w += gridDim.x) {
     const int it = w / a.nkv, kvh = w - it * a.nkv;
-    const int4 item = a.items[it];
+    const Item item = a.items[it];
     const int seq = item.x, k1 = min(item.z, a.bt_keys), qrow = item.w & 0xFFFFFF, nt = (item.w >> 24) + 1;
     const bool whole = item.y < 0;
     const int part = whole ? 0 : item.y, k0 = part * part_size;
@@ -700,7 +703,7 @@ K8S_API int k8s_int8_attn_reply(const void* q, long ldq, const void* k, const vo
   a.q = (const uint16_t*)q, a.ldq = ldq, a.k = (const uint8_t*)k, a.v = (const uint8_t*)v, a.ks = ks, a.vs = vs, a.bt = bt;
   a.bt_stride = bt_stride, a.bt_keys = (int)std::min((long)bt_cols * BS, 0x7fffffc0L), a.NB = NB, a.ctx = ctx, a.q_start = q_start, a.S = S, a.nq = nq, a.nkv = nkv, a.G = nq / nkv, a.BS = BS;
   a.scale_log2 = scale * kLog2e, a.out = (uint16_t*)out, a.ldo = ldo, a.part_o = part_o, a.part_ml = part_ml, a.n_parts = n_parts;
-  a.part_size = part_size, a.items = (const int4*)items, a.n_items = n_items, a.d_items = d_items;
+  a.part_size = part_size, a.items = (const Item*)items, a.n_items = n_items, a.d_items = d_items;
   hipStream_t st = (hipStream_t)stream;
   hipLaunchKernelGGL(reply_kernel, dim3(grid), dim3(64), 0, st, a);
   if (n_parts > 1) hipLaunchKernelGGL(reply_merge_kernel, dim3(nq, S), dim3(256), 0, st, a);

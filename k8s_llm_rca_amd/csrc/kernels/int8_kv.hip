@@ -104,7 +104,7 @@ __device__ __forceinline__ void rotate(const WriteArgs& a, int t, int part, int 
 // byte.  Column c of a dim is row c - (first row's slot mod 16), which lines the runs up.  us with the fours / without: 1055 rows of
 // 81 sequences, 16 + 2 x 16 heads, 14.5 / 21.5, 2652 of 22 17.1 / 22.4, 8000 of 5, 32 + 2 x 8 heads, 47.1 / 51.9.
 __device__ __forceinline__ void values(const WriteArgs& a, int t0, int head) {
-  __shared__ uint8_t sm[128 * kPitch];
+  __shared__ alignas(16) uint8_t sm[128 * kPitch];  // (read as words)
   __shared__ int slots[kCols], whole[kCols / 16], piece[kCols];
   __shared__ size_t first[kCols];  // where the column's first dim lies in the cache
   const int tid = threadIdx.x, j = tid & 7;

@@ -997,6 +997,17 @@ def test_pages_that_the_pool_does_not_have_count_as_the_nearest(device, lens, nq
     assert torch.equal(Q.paged_attention_int8(q, cache, meta, nq, nkv, 0.09), want)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("at", [1, 2, 3])
+def test_a_plan_s_lists_may_begin_at_any_word(at):
+    q, cache, meta, starts, ctx = attn_case("cuda", [(1, 900), (1, 300)], 8, 2)
+    planned(meta, starts, ctx, 8, 2, 64, part=64)
+    buf = torch.zeros(at + meta.items.numel(), dtype=torch.int32, device="cuda")
+    buf[at:] = meta.items.view(-1)
+    meta.items = buf[at:].view(-1, 4)
+    check_attention(Q.paged_attention_int8(q, cache, meta, 8, 2, 0.09), q, cache, meta, starts, ctx, 8, 2, 0.09)
+
+
 # ------------------------------------------------------------------ refusals
 def test_refusals():
     x, w = torch.randn(4, 64), torch.ones(64)
