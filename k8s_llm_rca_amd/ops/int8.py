@@ -44,18 +44,18 @@ _ROW_TYPES = (torch.bfloat16, torch.float32)
 
 
 _NO_GRADIENT = "the 8-bit operators have no gradients: detach the inputs or call under torch.no_grad()"
+_grad_enabled = torch.is_grad_enabled
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _inputs(*tensors) -> int:
     """One device for all, whose number this is (-1: the CPU); none that asks for a gradient or that a launch by address would miss."""
-    dev = tensors[0].get_device()
+    dev, grad = tensors[0].get_device(), _grad_enabled()
     for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"tensors on {tensors[0].device} and {t.device}")
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
+        if t is not None:
+            if t.get_device() != dev:
+                raise ValueError(f"tensors on {tensors[0].device} and {t.device}")
+            if grad and t.requires_grad:
                 raise RuntimeError(_NO_GRADIENT)
     if forward_ad._current_level >= 0:
         for t in tensors:
@@ -371,7 +371,8 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
         raise ValueError("the rows of block_tables overlap")
     if _transforms() is not None:
         _seen(t for t in vars(meta).values() if isinstance(t, torch.Tensor))
-    ctx, starts = _lengths(ctx, starts, S)
+    if ctx.dtype is not torch.int32 or starts.dtype is not torch.int32 or ctx.numel() < S or starts.numel() <= S or ctx.stride() != (1,) or starts.stride() != (1,):
+        ctx, starts = _lengths(ctx, starts, S)
     ldq = _pitch(q)
     if not ldq:
         raise ValueError("q's rows must be dense and start at multiples of 16 bytes")
@@ -404,10 +405,7 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
         raise ValueError(f"{G} query heads a key head: a tile takes {A.PF8_ROWS}")
     if meta.tile_seq is None or meta.tile_kv1 is None:
         raise ValueError("the step has no plan: attach_plan")
-    _on(dev, meta.pf_o, meta.pf_ml)
-    _listed(dev, meta.n_tiles, meta.tile_seq, meta.tile_tok0, meta.tile_len, meta.tile_kv0, meta.tile_kv1, meta.tile_slot)
-    if meta.n_merge:
-        _listed(dev, meta.n_merge, meta.m_tok0, meta.m_len, meta.m_slot0, meta.m_np)
+    _on(dev, meta.tile_seq, meta.pf_o, meta.pf_ml)
     part_o, part_ml, tiles, merged, own, runs = meta.pf_o, meta.pf_ml, meta.n_tiles, meta.n_merge, 0, 1
     if A.PF_ROWS % G or BS != 64:
         # Where heads or pages do not fit the bf16 cache's kernels the plan has tiles of about 64 rows over whole key ranges.  A workgroup
@@ -419,8 +417,12 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
         tiles, merged, rows = T // own + S, 0, own * G
         blocks, pages = tiles * nkv, bt.shape[1] * BS // 64
         runs = max(1, min(256 // blocks, pages // 5) if blocks <= 128 else min(512 // blocks, pages // 16))
-    elif meta.tile_tokens * G > A.PF8_ROWS:
-        raise ValueError(f"a plan whose tiles have {meta.tile_tokens} tokens, for fewer than {G} query heads a key head")
+    else:
+        if meta.tile_tokens * G > A.PF8_ROWS:
+            raise ValueError(f"a plan whose tiles have {meta.tile_tokens} tokens, for fewer than {G} query heads a key head")
+        _listed(dev, tiles, meta.tile_seq, meta.tile_tok0, meta.tile_len, meta.tile_kv0, meta.tile_kv1, meta.tile_slot)
+        if merged:
+            _listed(dev, merged, meta.m_tok0, meta.m_len, meta.m_slot0, meta.m_np)
     if merged or runs > 1:  # (a split tile's parts are tiles of the plan: no more than those, without a look at the device)
         rows_kept = (tiles * runs if own else meta.n_slots or tiles) * nkv * A.PF8_ROWS
         if own or not _room(part_o, part_ml, rows_kept):  # (none in the plan, or one for fewer key heads)
@@ -455,13 +457,11 @@ def _listed(dev: int, n: int, *lists) -> None:
     """A plan's lists: what the kernels read of them is there, one behind another."""
     for t in lists:
         if t is None:
-            if n > 0:
-                raise ValueError("a list of the step's plan is missing")
-            continue
-        if t.get_device() != dev:
-            _on(dev, t)
+            raise ValueError("a list of the step's plan is missing")
         if t.dtype is not torch.int32 or t.numel() < n or not t.is_contiguous():
             raise ValueError(f"a plan's list must be contiguous int32 of {n}, not {t.dtype} {list(t.shape)}")
+        if t.get_device() != dev:
+            raise ValueError(f"a plan on {t.device} for device {dev}")
 
 
 def _attention_plain(q, cache: Int8KV, meta: A.AttnMeta, nq, nkv, scale, out):

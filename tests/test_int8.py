@@ -878,7 +878,6 @@ def test_a_chunk_takes_room_of_its_own_where_the_plan_has_too_little(said):
 def test_lists_of_a_plan():
     n = torch.arange(12, dtype=torch.int32)
     Q._listed(-1, 12, n, n.view(3, 4))
-    Q._listed(-1, 0, n, None)
     Q._listed(-1, 6, n[6:])
     for count, t in ((13, n), (6, n[::2]), (4, n.long()), (4, n.float()), (1, None)):
         with pytest.raises(ValueError):
