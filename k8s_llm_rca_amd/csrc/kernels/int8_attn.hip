@@ -6,7 +6,7 @@
 //
 // Replies: a wave holds 16 rows (token, q head) of one kv head and walks 64 keys at a time, a run of keys of a list that the host
 // made (long contexts in parts, which meet in a second launch).  What bounds it is the cache's way from memory: 96 replies over 1500
-// to 6000 keys of 8 heads 147 + 5 us, 5.3 TB/s (a large copy moves 5.1); one reply over 5003 keys 7.6 + 4 us, which is
+// to 6000 keys of 8 heads 148 + 5 us, 5.3 TB/s (a large weight alone is read at 6.9); one reply over 5003 keys 8 + 4 us, which is
 // latency: loads, softmax and exchange of two chunks a wave, and the second launch.  v_mfma_f32_16x16x32_bf16, S^T = K Q^T:
 // row rho of key tile (u, t) is key 16 (rho >> 2) + 8 u + 4 t + (rho & 3), so that lane group g = lane >> 4 is left with the
 // scores of keys 16 g .. 16 g + 15, whose values of one dim are one 16-byte load, and weights go to the second product
@@ -75,7 +75,7 @@ __device__ __forceinline__ void load_q(State& st, const AttnArgs& a, long row, i
 
 // Keys [k0, k1) (k0 a multiple of 64) of one sequence; row lane & 15 sees keys below lim, every row those below kmin.
 // A chunk's keys and values make room for the next chunk's as soon as they are used, so that a wave always has 8 to 16 KB on the way.
-// They are read non-temporally: a page is read once a step (96 replies over 1500 to 6000 keys 146.6 us, otherwise 151.3).
+// They are read non-temporally: a page is read once a step (96 replies over 1500 to 6000 keys take 3 % less).
 __device__ __forceinline__ u32x4 once(const uint8_t* p) { return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)); }
 __device__ __forceinline__ void walk(State& st, const AttnArgs& a, const int* bt, int kvh, int k0, int k1, int kmin, int lim, int lane) {
   const int r = lane & 15, g = lane >> 4, n = (k1 - k0 + 63) >> 6;
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(256) reply_merge_kernel(AttnArgs a) {
 // scores take the registers that the weights have left, the staging beside its second half.  A fixed order of instructions holds it
 // together: left to the compiler, the products come first and the weights behind them.
 // us of four threads' chunks of up to 2048 tokens over 4000, 32 + 2 x 8 heads: page after page 585, in turns 576, in this order
-// 507, with a turn's first reads in front of its barrier 495 (890 TFLOP/s); a prompt of 8192 567 (969).  What bounds it is the
+// 507, with a turn's first reads in front of its barrier 495 to 509 by card (865 to 890 TFLOP/s); a prompt of 8192 567 to 585 (940 to 970).  What bounds it is the
 // vector unit beside the matrix unit: a turn's 250 vector instructions and 32 exponentials a wave take as long as its 32 products,
 // two waves a SIMD leave some 30 % of both to waits, and tiles of 60 to 94 pages fill 256 units unevenly.
 constexpr int kRows = 256, kPitch = 272;
@@ -701,7 +701,8 @@ K8S_API int k8s_int8_attn_reply(const void* q, long ldq, const void* k, const vo
   if (n_parts > 1 && (!part_o || !part_ml || part_size <= 0 || (part_size & 63))) return (int)hipErrorInvalidValue;
   AttnArgs a{};
   a.q = (const uint16_t*)q, a.ldq = ldq, a.k = (const uint8_t*)k, a.v = (const uint8_t*)v, a.ks = ks, a.vs = vs, a.bt = bt;
-  a.bt_stride = bt_stride, a.bt_keys = (int)std::min((long)bt_cols * BS, 0x7fffffc0L), a.NB = NB, a.ctx = ctx, a.q_start = q_start, a.S = S, a.nq = nq, a.nkv = nkv, a.G = nq / nkv, a.BS = BS;
+  a.bt_stride = bt_stride, a.bt_keys = (int)std::min((long)bt_cols * BS, 0x7fffffc0L);
+  a.NB = NB, a.ctx = ctx, a.q_start = q_start, a.S = S, a.nq = nq, a.nkv = nkv, a.G = nq / nkv, a.BS = BS;
   a.scale_log2 = scale * kLog2e, a.out = (uint16_t*)out, a.ldo = ldo, a.part_o = part_o, a.part_ml = part_ml, a.n_parts = n_parts;
   a.part_size = part_size, a.items = (const Item*)items, a.n_items = n_items, a.d_items = d_items;
   hipStream_t st = (hipStream_t)stream;
@@ -725,7 +726,8 @@ K8S_API int k8s_int8_attn_chunk(const void* q, long ldq, const void* k, const vo
   if (merged > 0 && (!part_o || !part_ml)) return (int)hipErrorInvalidValue;
   AttnArgs a{};
   a.q = (const uint16_t*)q, a.ldq = ldq, a.k = (const uint8_t*)k, a.v = (const uint8_t*)v, a.ks = ks, a.vs = vs, a.bt = bt;
-  a.bt_stride = bt_stride, a.bt_keys = (int)std::min((long)bt_cols * BS, 0x7fffffc0L), a.NB = NB, a.ctx = ctx, a.q_start = q_start, a.S = S, a.nq = nq, a.nkv = nkv, a.G = nq / nkv, a.BS = BS;
+  a.bt_stride = bt_stride, a.bt_keys = (int)std::min((long)bt_cols * BS, 0x7fffffc0L);
+  a.NB = NB, a.ctx = ctx, a.q_start = q_start, a.S = S, a.nq = nq, a.nkv = nkv, a.G = nq / nkv, a.BS = BS;
   a.scale_log2 = scale * kLog2e, a.out = (uint16_t*)out, a.ldo = ldo, a.part_o = part_o, a.part_ml = part_ml, a.own = own, a.parts = runs;
   a.tile_seq = tile_seq, a.tile_tok0 = tile_tok0, a.tile_len = tile_len, a.tile_kv0 = tile_kv0, a.tile_kv1 = tile_kv1, a.tile_slot = tile_slot;
   a.n_tiles = n_tiles, a.m_tok0 = m_tok0, a.m_len = m_len, a.m_slot0 = m_slot0, a.m_np = m_np;

@@ -138,8 +138,8 @@ __device__ __forceinline__ void put_turned(const GemmArgs& a, float* lds, int la
 
 // ------------------------------------------------------------ few rows: the weight streams by
 // A workgroup has 16 columns and up to 16 rows; its eight waves cut K into eight runs and meet in LDS.  What bounds it is the weight's
-// way: one row of 128256 x 4096 90 us (5.8 TB/s), 28672 x 4096 23.5, 6144 x 4096 8.2 (2 to 3 of them the launch); 16 rows read x
-// as often as w (141 us), so that others take over.  us of one row of 4096 x 4096 / 28672 x 4096 in other forms: eight steps asked
+// way: one row of 28672 x 4096 25 us (4.7 TB/s), of 6144 x 4096 8.2 (2 to 3 of them the launch), of 128256 x 4096 102 (5.1 TB/s); 16 rows
+// read x as often as w (143 us), so that others take over.  us of one row of 4096 x 4096 / 28672 x 4096 in other forms: eight steps asked
 // for at once 6.7 / 27.4, 16 waves 6.5 / 29.1, waves taking turns over K 6.4 / 30.5, two strips 7.6 / 31.0, non-temporal 5.6 / 24.6,
 // this one 5.8 / 23.2.
 constexpr int kWaves = 8;
@@ -209,8 +209,8 @@ __device__ __forceinline__ void put_part(const GemmArgs& a, int slice, int m, in
 
 // ------------------------------------------------------------ middle sizes: tiles of BM x BN behind a ring of stages
 // Waves 2 x WN; NB stages of 128 bytes of K, NB - 1 of them on their way while one is multiplied; one barrier a stage.  Up to
-// 128 rows the weight's way bounds it (48 rows of 128256 x 4096 108 us, 4.9 TB/s), from then on the stages' way into LDS (some 25
-// bytes a clock and unit): 256 x 4096 x 4096 13 us (660 TOP/s), 1024 x 4096 x 4096 24 us (1430).
+// 128 rows the weight's way bounds it (48 rows of 128256 x 4096 118 to 134 us, 4.1 to 4.7 TB/s), from then on the stages' way into
+// LDS (some 25 bytes a clock and unit): weights from memory, 256 x 4096 x 4096 17.6 us (490 TOP/s), 1024 x 4096 x 4096 28.8 (1190).
 template <int BM, int BN, int NB, int WN>
 __global__ void __launch_bounds__(128 * WN, 2) ring_kernel(GemmArgs a, int n_mt, int n_nt) {
   constexpr int STAGE = (BM + BN) * 128, I = (BM + BN) / (16 * WN);  // DMAs a wave and stage
@@ -222,8 +222,8 @@ __global__ void __launch_bounds__(128 * WN, 2) ring_kernel(GemmArgs a, int n_mt,
   tile_at(t0 / a.splits, n_mt, n_nt, tm, tn);
   const int m0 = tm * BM, n0 = tn * BN;
   const int all = (a.K + 127) >> 7, per = (all + a.splits - 1) / a.splits, kt0 = slice * per, nt = min(all - kt0, per);
-  // One row of tiles over an uncut K streams the weight by, and it need not stay in the caches: 17 and 48 rows of 128256 x 4096 99 -> 92
-  // and 112 -> 108 us, of 28672 x 4096 26.8 -> 25.0 and 29.7 -> 28.2 (with K in four runs 4096 x 14336 took longer: 16.4 -> 17.9).
+  // One row of tiles over an uncut K streams the weight by, and it need not stay in the caches: 17 and 48 rows of 128256 x 4096 take
+  // 7 and 4 % less, of 28672 x 4096 7 and 5 % (with K in four runs 4096 x 14336 took 9 % more).
   const bool once = n_mt == 1 && a.splits == 1;
 
   const uint8_t* src[I];
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(128 * WN, 2) ring_kernel(GemmArgs a, int n_mt,
 // read once a stage.  Waves 4-7 run one barrier behind waves 0-3, so that on each SIMD one wave multiplies while the other
 // reads.  A half tile is asked for two phases after its place was last read and waited for (four half tiles later still on
 // their way) one phase before it is read.  Rows of w are staged so that a lane's two fragments are eight neighbouring columns.
-// us: 4001 x 28672 x 4096 386 to 394 (2.40 POP/s), 4096 x 4096 x 14336 171 to 177 (2.75), 4096 x 4096 x 4096 56 (2.45); a large bf16
+// us: 4001 x 28672 x 4096 386 to 414 (2.27 to 2.43 POP/s), 4096 x 4096 x 14336 177 to 180 (2.7), 4096 x 4096 x 4096 59 to 62 (2.3); a large bf16
 // product of the library reaches 1.46 PFLOP/s, whose bytes a matrix instruction are the same.  A stage takes 1.5 us, of which the
 // matrix instructions are 1.0: LDS moves as much in the time as it can (192 KB read, 64 KB written a stage); 6 us of each tile
 // are its start and its stores.  What whole rounds of 256 tiles leave has its K cut: 2048 x 10240 x 8192 (320 tiles) 185 -> 155.
@@ -471,9 +471,10 @@ constexpr int kEdge[8][2] = {{16, 16}, {32, 64}, {64, 64}, {64, 128}, {128, 64},
 // rows' reads beside it, against the latency of each wave's turns over K (four steps of 64 bytes a turn), and what a workgroup
 // costs beside its loads, which shows where K is short.  The constants are a fit to times of every kind and cut at 480 sizes: 1 to
 // 4096 rows by 16 weights of 512 x 512 to 128256 x 4096 (K from 512 to 28672), the weights from memory.  The choice is 1.3 % from
-// the best one on average; furthest off are 13 and 16 rows of 5120 x 5120, 14.6 and 16.0 us for 10.9.
-// Tiles of 128 x 256 came later (96 sizes, 72 to 1000 rows: 0.4 % from the best one, without them 4.1; 512 rows of 14336 x 4096 46.6 -> 38.4 us,
-// 128 of 40000 x 4096 54.9 -> 46.6, 256 of 28672 x 4096 48.4 -> 43.4, 100 of 128256 x 4096 134 -> 126).
+// the best one on average; furthest off are 13 and 16 rows of 5120 x 5120, 16.0 and 17.2 us where
+// 32 x 64 tiles in four runs take 14.1, and one row of 128256 x 4096, which goes to tiles, 120 us for 102.
+// Tiles of 128 x 256 came later (96 sizes, 72 to 1000 rows: 0.4 % from the best one, without them 4.1; 512 rows of 14336 x 4096 take
+// 18 % less, 41 us, 128 of 40000 x 4096 15 %, 256 of 28672 x 4096 10 %, 100 of 128256 x 4096 6 %).
 inline double cost(int M, int N, int K, int kind, int splits) {
   constexpr double kStart = 2.62, kByte = 0.150e-6, kJoin = 2.46, kJoinByte = 0.328e-6;
   // us a stage alone on a unit, by twos (of the three largest, a round full and nearly empty), a round's fixed part

@@ -5,8 +5,8 @@
 // One pass over memory: a row stays in the registers of its threads between its maximum and its integers (rows too long for that are
 // read again).  Behind a norm the sum of squares and the maximum of |h w| leave in one exchange: the norm's factor is the
 // same for the whole row, so it does not change the integers, only the scale.
-// What bounds it is memory: a norm of 8192 x 8192 bf16 with its residual 78 to 88 us (470 MB: 5.3 to 6.0 TB/s; a large copy moves
-// 5.1), a gate of 4096 x 14336 53 us (5.5 TB/s); a few rows are 3 us of launch, load and exchange.
+// What bounds it is memory: a norm of 8192 x 8192 bf16 with its residual 87 to 92 us (470 MB: 5.1 to 5.4 TB/s; a large copy moves
+// 5.1, of which it reads a smaller part), a gate of 4096 x 14336 53 us (5.5 TB/s); a few rows are 3 us of launch, load and exchange.
 #include "int8_rows.h"
 
 namespace k8s {
@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(W >= 4 ? 64 * W : 256) rows_kernel(RowArgs a) 
       float u[8];
       load8(x + 8 * i, y);
       load8(x + a.H + 8 * i, u);
-      // (the quotient by the approximate reciprocal: 2^-22, a thousandth of a thousandth of an integer's step)
+      // (hardware exponential and reciprocal: y and the maximum are off by 2^-18 at most, an integer by a thousandth of its step)
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] = silu_hw(y[j]) * u[j];
     } else if constexpr (MODE == NORM) {
@@ -164,8 +164,9 @@ __global__ void __launch_bounds__(W >= 4 ? 64 * W : 256) rows_kernel(RowArgs a) 
   }
 }
 
-// Waves a row.  Few rows wait for their own loads and exchange: a piece a lane, two at most.  Many rows fill the chip by themselves:
-// fewer waves a row, up to four pieces a lane.  us of a norm with its residual, bf16, at 32 / 8192 rows: 1024 wide by 1 wave
+// Waves a row.  Few rows wait for their own loads and exchange: a piece a lane, two up to 8192 wide, up to four beyond that.  Many rows fill
+// the chip by themselves: fewer waves a row, up to four pieces a lane.  us of a norm with its residual, bf16, the same rows again and
+// again, at 32 / 8192 rows: 1024 wide by 1 wave
 // 3.7 / 10.0, by 4 3.2 / 16.0; 2048 wide by 1 4.7 / 19.7, by 4 3.2 / 22.2; 4096 wide by 4 3.8 / 37.0, by 8 3.3 / 38.4; 8192 wide by 4
 // 4.9 / 77.8, by 8 3.9 / 77.2, by 16 3.9 / 82.1; 14336 wide by 8 4.8 / 156, by 16 4.5 / 152.
 template <int MODE, typename E>

@@ -411,8 +411,8 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
         # Where heads or pages do not fit the bf16 cache's kernels the plan has tiles of about 64 rows over whole key ranges.  A workgroup
         # here takes 256 rows and finds them by itself.  Few of them cut their keys until there are as many as compute units, of
         # five pages each at least; from half as many on they make two rounds, which even out short and long tiles.  us by the plan's
-        # tiles and by these, 10 + 2 x 2 heads: six threads' six tokens over 8064 keys 260 and 27, a prompt of 4096 225 and 97, two
-        # of 513 27 and 26; 12 + 2 x 4: two chunks of 2000 over 2000 273 and 114, six prompts of 234 17.7 and 18.4.
+        # tiles and by these, 10 + 2 x 2 heads: six threads' six tokens over 8064 keys 260 and 23, a prompt of 4096 225 and 101, two
+        # of 513 27 and 26; 12 + 2 x 4: two chunks of 2000 over 2000 273 and 118, six prompts of 234 17.7 and 18.4.
         own = min(A.PF8_ROWS // G, T)
         tiles, merged, rows = T // own + S, 0, own * G
         blocks, pages = tiles * nkv, bt.shape[1] * BS // 64
