@@ -348,8 +348,9 @@ def paged_attention_int8(q: torch.Tensor, cache: Int8KV, meta: A.AttnMeta, nq: i
                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of ``q`` [T, >= nq 128] (row stride free) over the 8-bit pages -> [T, nq 128], for reply tokens and
     chunks alike.  ``meta`` is the step's, with the plan that ``attention.paged_attention`` takes (``attach_decode_plan`` or
-    ``attach_plan``): one plan serves both caches.  A row without a visible key gives zeros.  A context ends
-    where its row of the table does; a page that the pool does not have counts as its nearest one."""
+    ``attach_plan``): one plan serves both caches.  A plan for fewer heads, or whose lists or reply workspace are too short, is
+    refused; a chunk's parts take a workspace of their own where the plan has none that holds them.  A row without a visible key
+    gives zeros.  A context ends where its row of the table does; a page that the pool does not have counts as its nearest one."""
     T = q.shape[0]
     _heads(q, cache, nq, nkv, nq * HEAD_DIM, "q")
     NB, _, BS, D = cache.k.shape
